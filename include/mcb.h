@@ -596,6 +596,124 @@ MCB_API mcb_status mcb_device_zero(mcb_buffer handle) MCB_NOEXCEPT;
 MCB_API mcb_status mcb_device_zero_raw_on_stream(void *device_ptr, uint64_t size_bytes,
                                                  void *stream) MCB_NOEXCEPT;
 
+/* ---- serving: a paged key/value cache and what reads and follows it ------------
+ * None of these has a counterpart in the reference. All operands live in
+ * device memory (MCB_STATUS_UNSUPPORTED_MEMORY_SPACE otherwise); a call is
+ * asynchronous on the stream unless MCB_EXEC_SYNC is set, never reads a
+ * length on the host, and can be captured into a CUDA graph. Index tensors
+ * (lengths, tables, slots, positions, token ids) are i32. What a length or an
+ * index on the device says is checked where it is used: the result for values
+ * out of range is stated below and nothing outside the tensors is touched. Negative
+ * lengths count as 0. Outputs may not overlap inputs except where stated
+ * (MCB_STATUS_ALIAS_VIOLATION).
+ *
+ * A cache is two tensors K, V [blocks, block, kv_heads, dim]; a request's token
+ * at position p lives in block table[request, p / block], row p % block, its
+ * slot number being table[request, p / block] * block + p % block. */
+
+/* Grows requests by new_lens[b] tokens each, in order, taking cache blocks
+ * from the top of the stack free_blocks[0 .. free_count[0]).
+ *   block_table [B, columns] (rows may be strided): entries of new blocks are written;
+ *   slots [T], positions [T]: cache slot and position of each new token, the
+ *     tokens of request b at cu_new[b] .. cu_new[b+1]; entries from
+ *     cu_new[B] on are -1 and 0;
+ *   cu_new [B+1]: prefix sums of new_lens; len_after [B]; free_left [1].
+ * A request is refused as a whole when its blocks do not fit into a table row,
+ * when the blocks wanted up to and including its own exceed the stack (a
+ * request that wants no block is not refused), or when its tokens end past T:
+ * its length stays, its slots are -1, no block is taken for it. The stack
+ * itself is not written: the next call is given free_left as its free_count. */
+MCB_API mcb_status mcb_paged_grow_v1(const mcb_tensor *block_table, const mcb_tensor *slots,
+                                     const mcb_tensor *positions, const mcb_tensor *cu_new,
+                                     const mcb_tensor *len_after, const mcb_tensor *free_left,
+                                     const mcb_tensor *lens, const mcb_tensor *new_lens,
+                                     const mcb_tensor *free_blocks,
+                                     const mcb_tensor *free_count, int64_t block,
+                                     const mcb_exec *exec) MCB_NOEXCEPT;
+/* Cuts requests from lens[b] to keep_lens[b] tokens (a keep at or above the
+ * length keeps all): the blocks of a request past its first
+ * ceil(keep / block) are pushed on the stack free_blocks in request order,
+ * from free_blocks[free_count[0]] on, as far as its capacity goes; free_left
+ * [1] is the new count. Block table rows are not written. */
+MCB_API mcb_status mcb_paged_release_v1(const mcb_tensor *free_blocks, const mcb_tensor *free_left,
+                                        const mcb_tensor *block_table, const mcb_tensor *lens,
+                                        const mcb_tensor *keep_lens, const mcb_tensor *free_count,
+                                        int64_t block, const mcb_exec *exec) MCB_NOEXCEPT;
+
+/* Rotary positions: pair i < R of every head of q [T, heads, dim] and k [T,
+ * kv_heads, dim] is turned by the angle whose cosine and sine stand in
+ * cos_sin [rows, 2R] (f32; cos of pairs 0..R-1, then sin) at row
+ * positions[axis_map[i], t]; elements from 2R on are copied. Pairs are
+ * (x[i], x[R+i]), or with MCB_ROPE_PAIRED (x[2i], x[2i+1]).
+ * MCB_ROPE_INVERSE turns back, which is the gradient of the rotation.
+ * positions is [T] or [axes, T], axes <= 4; axis_map (R bytes in host memory,
+ * read during the call) may be NULL for axis 0 everywhere; R <= 128. q, k and
+ * the outputs share one type (f32, bf16, f16); products and sums are f32,
+ * rounded once. A position outside [0, rows) gives NaN in the turned elements.
+ * q_out may be q itself and k_out k itself (same base and strides). */
+enum { MCB_ROPE_PAIRED = 1u << 0, MCB_ROPE_INVERSE = 1u << 1 };
+MCB_API mcb_status mcb_rope_v1(const mcb_tensor *q_out, const mcb_tensor *k_out,
+                               const mcb_tensor *q, const mcb_tensor *k,
+                               const mcb_tensor *cos_sin, const mcb_tensor *positions,
+                               const uint8_t *axis_map, uint32_t flags,
+                               const mcb_exec *exec) MCB_NOEXCEPT;
+/* The same with the turned k and v [T, kv_heads, dim] written to row slots[t]
+ * of the caches [blocks, block, kv_heads, dim] of the same type (any strides
+ * with unit innermost; blocks * block < 2^31). A slot outside the cache (-1 by
+ * convention) writes nothing; two tokens with one slot leave either. */
+MCB_API mcb_status mcb_rope_append_v1(const mcb_tensor *q_out, const mcb_tensor *k_cache,
+                                      const mcb_tensor *v_cache, const mcb_tensor *q,
+                                      const mcb_tensor *k, const mcb_tensor *v,
+                                      const mcb_tensor *cos_sin, const mcb_tensor *positions,
+                                      const mcb_tensor *slots, const uint8_t *axis_map,
+                                      uint32_t flags, const mcb_exec *exec) MCB_NOEXCEPT;
+
+/* Attention of new (drafted) tokens over a paged cache that already holds
+ * their keys and values: o [T, heads, dim] = softmax(scale q k^T) v and, when
+ * lse is given, lse [T, heads] (f32) = log of the softmax's sum. Request b
+ * owns tokens cu_new[b] .. cu_new[b+1] (n of them) and kv_lens[b] keys, the
+ * last n of which are its new tokens'. A token sees every key before those
+ * and, of the new ones, those whose bit is set in its row of tree_mask
+ * [T, words] (i32; bit j % 32 of word j / 32 is new token j of the request; bits past
+ * the words are 0); with tree_mask NULL token i sees j <= i, so n = 1 is
+ * plain decoding. heads is a multiple of kv_heads. A row that sees no key (and
+ * a token of no request) gives o = 0, lse = -inf; keys past the table's
+ * columns and of table entries outside the cache are not seen. What is not
+ * seen has no influence, NaN and infinities included.
+ * q, o and the caches share one type (bf16, f16, f32), dim <= 256. bf16 and
+ * f16 with dim 64 or 128 and 16-byte aligned bases and strides run on
+ * tcgen05 (the weights rounded to the 16-bit type for the second product,
+ * statistics and sums in f32), all else on CUDA cores in f32. Scratch for
+ * partial results of long contexts: see Scratch above. */
+MCB_API mcb_status mcb_tree_attention_v1(const mcb_tensor *o, const mcb_tensor *lse,
+                                         const mcb_tensor *q, const mcb_tensor *k_cache,
+                                         const mcb_tensor *v_cache,
+                                         const mcb_tensor *block_table,
+                                         const mcb_tensor *cu_new, const mcb_tensor *kv_lens,
+                                         const mcb_tensor *tree_mask, double scale,
+                                         const mcb_exec *exec) MCB_NOEXCEPT;
+
+/* Penalties for repeated tokens, biases and a grammar mask on logits [R, V]
+ * (f32, bf16, f16) into out [R, V] (f32 or the logits' type; out may be the
+ * logits themselves, same base, strides and type). Row r's history is
+ * token_ids[cu_tokens[r] .. cu_tokens[r+1]), its first prompt_lens[r] the
+ * prompt, the rest generated. In f32, in this order, rounded once:
+ *   v in the history:   x = x > 0 ? x / repetition[r] : x * repetition[r]
+ *   v generated n > 0 times: x = x - frequency[r] * n - presence[r]
+ *   v in the row's list bias_ids[bias_cu[r] .. bias_cu[r+1]):
+ *                       x = x + its bias_values entry (its last, if several)
+ *   bit v of row r of allowed [R, ceil(V/32)] (i32) clear: x = -inf
+ * Any of repetition, presence, frequency [R] f32, the three bias tensors
+ * (together) and allowed may be NULL. Ids outside [0, V) are ignored. */
+MCB_API mcb_status mcb_adjust_logits_v1(const mcb_tensor *out, const mcb_tensor *logits,
+                                        const mcb_tensor *token_ids, const mcb_tensor *cu_tokens,
+                                        const mcb_tensor *prompt_lens,
+                                        const mcb_tensor *repetition, const mcb_tensor *presence,
+                                        const mcb_tensor *frequency, const mcb_tensor *bias_ids,
+                                        const mcb_tensor *bias_values, const mcb_tensor *bias_cu,
+                                        const mcb_tensor *allowed,
+                                        const mcb_exec *exec) MCB_NOEXCEPT;
+
 /* ---- test support: host-side fault injection ------------------------------
  * The counterpart of the reference's fake-driver adapter test
  * (compiler/tests/generated_gpu/cuda_adapter_test.cpp): a table of stand-ins

@@ -33,6 +33,7 @@ BIAS_MODE = {"none": 0, "row": 1, "full": 2}
 BIAS_OP = {"add": 0, "rsub": 1}
 ACT = {"none": 0, "relu": 1, "gelu_tanh": 2, "exp": 3, "sigmoid": 4, "tanh": 5}
 GEMM_W_TRANSPOSED = 1
+ROPE_PAIRED, ROPE_INVERSE = 1, 2
 
 
 class Tensor(ctypes.Structure):
@@ -184,6 +185,12 @@ SIGNATURES = {
     "mcb_attn_block_heads_pair_v1": (ctypes.c_int32, [_T, _T, _T, _T, _T, _T, ctypes.c_int64,
                                                       ctypes.c_float, ctypes.c_int32,
                                                       ctypes.c_void_p, _E]),
+    "mcb_paged_grow_v1": (ctypes.c_int32, [_T] * 10 + [ctypes.c_int64, _E]),
+    "mcb_paged_release_v1": (ctypes.c_int32, [_T] * 6 + [ctypes.c_int64, _E]),
+    "mcb_rope_v1": (ctypes.c_int32, [_T] * 6 + [ctypes.c_char_p, ctypes.c_uint32, _E]),
+    "mcb_rope_append_v1": (ctypes.c_int32, [_T] * 9 + [ctypes.c_char_p, ctypes.c_uint32, _E]),
+    "mcb_tree_attention_v1": (ctypes.c_int32, [_T] * 9 + [ctypes.c_double, _E]),
+    "mcb_adjust_logits_v1": (ctypes.c_int32, [_T] * 12 + [_E]),
     "mcb_plan_create_v1": (ctypes.c_int32, [_P(PlanDesc), _P(ctypes.c_void_p)]),
     "mcb_plan_execute_v1": (ctypes.c_int32, [ctypes.c_void_p, _T, ctypes.c_uint32,
                                              ctypes.c_void_p]),

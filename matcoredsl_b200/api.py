@@ -436,6 +436,122 @@ def residual_rmsnorm(x, p, eps=1e-6, out=None, *, device=-1, flags=0):
     return out
 
 
+def paged_grow(block_table, lens, new_lens, free_blocks, free_count, block, *, tokens=None, out=None,
+               device=-1, flags=0):
+    """Grows the requests of a paged cache by new_lens[b] tokens each
+    (mcb_paged_grow_v1): writes the new blocks into block_table [B, columns]
+    and returns (slots [tokens], positions [tokens], cu_new [B+1], len_after
+    [B], free_left [1]), all int32. `tokens` is the room for new tokens (their
+    exact number, or more); `out` holds the five results instead."""
+    if out is None:
+        if tokens is None:
+            raise ValueError("paged_grow: give `tokens`, the room for new tokens, or `out`")
+        e = lambda n: _torch().empty(n, dtype=_torch().int32, device=lens.device)  # noqa: E731
+        b = lens.shape[0]
+        out = (e(tokens), e(tokens), e(b + 1), e(b), e(1))
+    slots, positions, cu_new, len_after, free_left = out
+    _call("mcb_paged_grow_v1",
+          [("block_table", block_table), ("slots", slots), ("positions", positions),
+           ("cu_new", cu_new), ("len_after", len_after), ("free_left", free_left), ("lens", lens),
+           ("new_lens", new_lens), ("free_blocks", free_blocks), ("free_count", free_count)],
+          [int(block)], device, flags)
+    return out
+
+
+def paged_release(block_table, lens, keep_lens, free_blocks, free_count, block, *, out=None,
+                  device=-1, flags=0):
+    """Cuts requests to keep_lens[b] tokens (mcb_paged_release_v1): pushes the
+    blocks they no longer need on the stack free_blocks and returns its new
+    count, free_left [1]."""
+    if out is None:
+        out = _torch().empty(1, dtype=_torch().int32, device=lens.device)
+    _call("mcb_paged_release_v1",
+          [("free_blocks", free_blocks), ("free_left", out), ("block_table", block_table),
+           ("lens", lens), ("keep_lens", keep_lens), ("free_count", free_count)], [int(block)],
+          device, flags)
+    return out
+
+
+def _rope_args(cos_sin, axis_map, paired, inverse):
+    if axis_map is not None:
+        axis_map = bytes(axis_map)
+        if 2 * len(axis_map) != cos_sin.shape[-1]:
+            raise ValueError("axis_map: one axis for each of cos_sin's pairs")
+    return [axis_map, (_abi.ROPE_PAIRED if paired else 0) | (_abi.ROPE_INVERSE if inverse else 0)]
+
+
+def rope(q, k, cos_sin, positions, *, axis_map=None, paired=False, inverse=False, out=None,
+         device=-1, flags=0):
+    """Rotary positions on q [T, heads, dim] and k [T, kv_heads, dim]
+    (mcb_rope_v1). cos_sin [rows, 2R] f32 holds cos then sin of R pairs at each
+    position; positions is [T] or [axes, T]; axis_map (R small numbers) says
+    whose position turns each pair. `inverse` is the rotation's gradient.
+    `out` may be (q, k) themselves. Returns (q_out, k_out)."""
+    if out is None:
+        e = lambda t: _torch().empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
+        out = (e(q), e(k))
+    _call("mcb_rope_v1",
+          [("q_out", out[0]), ("k_out", out[1]), ("q", q), ("k", k), ("cos_sin", cos_sin),
+           ("positions", positions)], _rope_args(cos_sin, axis_map, paired, inverse), device, flags)
+    return out
+
+
+def rope_append(q, k, v, cos_sin, positions, slots, k_cache, v_cache, *, axis_map=None,
+                paired=False, out=None, device=-1, flags=0):
+    """rope() with the turned k and v [T, kv_heads, dim] written to row
+    slots[t] of the caches [blocks, block, kv_heads, dim]
+    (mcb_rope_append_v1; a slot outside the cache writes nothing). Returns
+    q_out."""
+    if out is None:
+        out = _torch().empty(q.shape, dtype=q.dtype, device=q.device)
+    _call("mcb_rope_append_v1",
+          [("q_out", out), ("k_cache", k_cache), ("v_cache", v_cache), ("q", q), ("k", k),
+           ("v", v), ("cos_sin", cos_sin), ("positions", positions), ("slots", slots)],
+          _rope_args(cos_sin, axis_map, paired, False), device, flags)
+    return out
+
+
+def tree_attention(q, k_cache, v_cache, block_table, cu_new, kv_lens, tree_mask=None, *,
+                   scale=None, out=None, lse=None, device=-1, flags=0, workspace=None):
+    """Attention of drafted tokens q [T, heads, dim] over a paged cache
+    (mcb_tree_attention_v1): request b owns tokens cu_new[b]..cu_new[b+1], the
+    last of its kv_lens[b] keys. tree_mask [T, words] int32: bit j of a row is
+    set where the token sees its request's j-th new token; None is causal.
+    scale defaults to dim^-0.5. `lse` [T, heads] f32 takes the logarithms of
+    the sums. Returns out."""
+    if out is None:
+        out = _torch().empty(q.shape, dtype=q.dtype, device=q.device)
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    _call("mcb_tree_attention_v1",
+          [("o", out), ("lse", lse), ("q", q), ("k_cache", k_cache), ("v_cache", v_cache),
+           ("block_table", block_table), ("cu_new", cu_new), ("kv_lens", kv_lens),
+           ("tree_mask", tree_mask)], [float(scale)], device, flags, workspace)
+    return out
+
+
+def adjust_logits(logits, token_ids, cu_tokens, prompt_lens, *, repetition=None, presence=None,
+                  frequency=None, bias_ids=None, bias_values=None, bias_cu=None, allowed=None,
+                  out=None, out_dtype=None, device=-1, flags=0):
+    """Penalties for repeated tokens, biases and a grammar mask on logits
+    [R, V] (mcb_adjust_logits_v1). Row r's history is
+    token_ids[cu_tokens[r]:cu_tokens[r+1]], its first prompt_lens[r] the
+    prompt. `out` may be the logits themselves; out_dtype "f32" widens."""
+    if out is None:
+        dt = logits.dtype if out_dtype is None else _torch().float32
+        if out_dtype not in (None, "f32", _torch_dtype_names().get(logits.dtype)):
+            raise ValueError("out_dtype: f32 or the logits' type")
+        if out_dtype is not None and out_dtype != "f32":
+            dt = logits.dtype
+        out = _torch().empty(logits.shape, dtype=dt, device=logits.device)
+    _call("mcb_adjust_logits_v1",
+          [("out", out), ("logits", logits), ("token_ids", token_ids), ("cu_tokens", cu_tokens),
+           ("prompt_lens", prompt_lens), ("repetition", repetition), ("presence", presence),
+           ("frequency", frequency), ("bias_ids", bias_ids), ("bias_values", bias_values),
+           ("bias_cu", bias_cu), ("allowed", allowed)], [], device, flags)
+    return out
+
+
 class Plan:
     """Shape-locked operator call with optional CUDA-graph replay (the
     reference's create_plan / execute_plan). Tensors are passed in the entry

@@ -43,6 +43,10 @@ SOURCES = {
     "typed.cu": [],
     "comm.cpp": [],
     "peer.cu": [],
+    "paged.cu": [],
+    "rope.cu": [],
+    "tree_attn.cu": [],
+    "logits.cu": [],
 }
 HEADERS = ["common.cuh", "internal.h", "epilogue.cuh"]
 

@@ -1943,6 +1943,416 @@ bool live(const mcb_buffer &h) {
          it->second.size_bytes == h.size_bytes && it->second.device == h.device;
 }
 
+// ---- serving: paged cache, rotary positions, tree attention, logits -------------------------
+// Device-resident operands only: lengths and indexes stay on the GPU.
+bool f_16_32(mcb_dtype t) {
+  return t == MCB_DTYPE_F32 || t == MCB_DTYPE_BF16 || t == MCB_DTYPE_F16;
+}
+mcb_status on_device(std::initializer_list<const mcb_tensor *> ts) {
+  for (const mcb_tensor *t : ts)
+    if (t && t->memory_space != MCB_MEMORY_CUDA_DEVICE) return MCB_STATUS_UNSUPPORTED_MEMORY_SPACE;
+  return MCB_STATUS_OK;
+}
+// A vector of `n` entries (any number when n < 0).
+mcb_status check_vector(const mcb_tensor *t, mcb_dtype dtype, int64_t n) {
+  const mcb_status s = check_tensor(t, 1, 1);
+  if (s) return s;
+  if (t->dtype != dtype) return MCB_STATUS_UNSUPPORTED_DTYPE;
+  if (n >= 0 && t->dims[0] != n) return MCB_STATUS_SHAPE_MISMATCH;
+  return MCB_STATUS_OK;
+}
+bool same_place(const mcb_tensor *a, const mcb_tensor *b) {
+  if (a->data != b->data || a->dtype != b->dtype || a->rank != b->rank) return false;
+  for (uint32_t i = 0; i < a->rank; ++i)
+    if (a->dims[i] != b->dims[i] || (a->dims[i] > 1 && a->strides[i] != b->strides[i]))
+      return false;
+  return true;
+}
+// Whether two [T, heads, dim] views share an element, for views whose rows
+// interleave too (q, k and v of one packed projection): with equal row strides
+// they are apart when each row's spans are, modulo the stride.
+bool views_overlap(const mcb_tensor *a, const mcb_tensor *b) {
+  if (!overlaps(a, b)) return false;
+  if (a->rank != 3 || b->rank != 3 || a->dtype != b->dtype || a->strides[0] != b->strides[0])
+    return true;
+  const int64_t es = static_cast<int64_t>(dtype_size(a->dtype)), row = a->strides[0];
+  auto width = [](const mcb_tensor *t) { return (t->dims[1] - 1) * t->strides[1] + t->dims[2]; };
+  if (width(a) > row || width(b) > row) return true;
+  const int64_t apart = static_cast<const char *>(b->data) - static_cast<const char *>(a->data);
+  if (apart % es != 0) return true;
+  const int64_t off = ((apart / es) % row + row) % row;
+  return !(off >= width(a) && off + width(b) <= row);
+}
+const int32_t *i32(const mcb_tensor *t) { return t ? static_cast<const int32_t *>(t->data) : nullptr; }
+int32_t *i32_out(const mcb_tensor *t) { return static_cast<int32_t *>(t->data); }
+const float *f32(const mcb_tensor *t) { return t ? static_cast<const float *>(t->data) : nullptr; }
+
+mcb_status paged_table_args(const mcb_tensor *table, const mcb_tensor *lens,
+                            const mcb_tensor *other_lens, const mcb_tensor *free_blocks,
+                            const mcb_tensor *free_count, const mcb_tensor *free_left,
+                            int64_t block) {
+  mcb_status s;
+  if ((s = check_tensor(table, 2, 2))) return s;
+  if (table->dtype != MCB_DTYPE_I32) return MCB_STATUS_UNSUPPORTED_DTYPE;
+  const int64_t B = table->dims[0];
+  if ((s = check_vector(lens, MCB_DTYPE_I32, B)) ||
+      (s = check_vector(other_lens, MCB_DTYPE_I32, B)) ||
+      (s = check_vector(free_blocks, MCB_DTYPE_I32, -1)) ||
+      (s = check_vector(free_count, MCB_DTYPE_I32, 1)) ||
+      (s = check_vector(free_left, MCB_DTYPE_I32, 1)))
+    return s;
+  if (block < 1 || block > 0x7fffffff) return MCB_STATUS_INVALID_ARGUMENT;
+  if (B > 0x7fffffff || table->dims[1] > 0x7fffffff) return MCB_STATUS_INVALID_SHAPE;
+  return MCB_STATUS_OK;
+}
+
+mcb_status paged_grow_impl(const mcb_tensor *table, const mcb_tensor *slots,
+                           const mcb_tensor *positions, const mcb_tensor *cu,
+                           const mcb_tensor *after, const mcb_tensor *free_left,
+                           const mcb_tensor *lens, const mcb_tensor *new_lens,
+                           const mcb_tensor *free_blocks, const mcb_tensor *free_count,
+                           int64_t block, const mcb_exec *exec) {
+  mcb_status s = paged_table_args(table, lens, new_lens, free_blocks, free_count, free_left, block);
+  if (s) return s;
+  const int64_t B = table->dims[0];
+  if ((s = check_vector(slots, MCB_DTYPE_I32, -1)) ||
+      (s = check_vector(positions, MCB_DTYPE_I32, slots->dims[0])) ||
+      (s = check_vector(cu, MCB_DTYPE_I32, B + 1)) || (s = check_vector(after, MCB_DTYPE_I32, B)))
+    return s;
+  if ((s = on_device({table, slots, positions, cu, after, free_left, lens, new_lens, free_blocks,
+                      free_count})))
+    return s;
+  const mcb_tensor *outs[] = {table, slots, positions, cu, after, free_left};
+  for (int i = 0; i < 6; ++i) {
+    for (int j = i + 1; j < 6; ++j)
+      if (overlaps(outs[i], outs[j])) return MCB_STATUS_ALIAS_VIOLATION;
+    for (const mcb_tensor *t : {lens, new_lens, free_blocks, free_count})
+      if (overlaps(outs[i], t)) return MCB_STATUS_ALIAS_VIOLATION;
+  }
+  Call call(exec);
+  if ((s = call.begin(false))) return s;
+  mcb::PagedGrow p;
+  p.table = i32_out(table);
+  p.slots = i32_out(slots);
+  p.positions = i32_out(positions);
+  p.cu = i32_out(cu);
+  p.after = i32_out(after);
+  p.free_left = i32_out(free_left);
+  p.lens = i32(lens);
+  p.new_lens = i32(new_lens);
+  p.free = i32(free_blocks);
+  p.free_count = i32(free_count);
+  p.requests = B;
+  p.columns = table->dims[1];
+  p.table_stride = table->strides[0];
+  p.tokens = slots->dims[0];
+  p.free_capacity = free_blocks->dims[0];
+  p.block = static_cast<int32_t>(block);
+  LaunchInfo info;
+  call.mark_compute_start();
+  const cudaError_t err = mcb::launch_paged_grow(p, call.stream(), &info);
+  call.mark_compute_end();
+  if (err == cudaErrorNotSupported) return MCB_STATUS_UNAVAILABLE_VARIANT;
+  return call.finish(nullptr, nullptr, info, err);
+}
+
+mcb_status paged_release_impl(const mcb_tensor *free_blocks, const mcb_tensor *free_left,
+                              const mcb_tensor *table, const mcb_tensor *lens,
+                              const mcb_tensor *keep_lens, const mcb_tensor *free_count,
+                              int64_t block, const mcb_exec *exec) {
+  mcb_status s = paged_table_args(table, lens, keep_lens, free_blocks, free_count, free_left, block);
+  if (s) return s;
+  if ((s = on_device({free_blocks, free_left, table, lens, keep_lens, free_count}))) return s;
+  for (const mcb_tensor *o : {free_blocks, free_left})
+    for (const mcb_tensor *t : {table, lens, keep_lens, free_count})
+      if (overlaps(o, t)) return MCB_STATUS_ALIAS_VIOLATION;
+  if (overlaps(free_blocks, free_left)) return MCB_STATUS_ALIAS_VIOLATION;
+  Call call(exec);
+  if ((s = call.begin(false))) return s;
+  mcb::PagedRelease p;
+  p.free = i32_out(free_blocks);
+  p.free_left = i32_out(free_left);
+  p.table = i32(table);
+  p.lens = i32(lens);
+  p.keep_lens = i32(keep_lens);
+  p.free_count = i32(free_count);
+  p.requests = table->dims[0];
+  p.columns = table->dims[1];
+  p.table_stride = table->strides[0];
+  p.free_capacity = free_blocks->dims[0];
+  p.block = static_cast<int32_t>(block);
+  LaunchInfo info;
+  call.mark_compute_start();
+  const cudaError_t err = mcb::launch_paged_release(p, call.stream(), &info);
+  call.mark_compute_end();
+  if (err == cudaErrorNotSupported) return MCB_STATUS_UNAVAILABLE_VARIANT;
+  return call.finish(nullptr, nullptr, info, err);
+}
+
+// A cache pair [blocks, block, kv_heads, dim] of one type and shape.
+mcb_status check_caches(const mcb_tensor *k, const mcb_tensor *v, int64_t kv_heads, int64_t dim,
+                        mcb_dtype dtype) {
+  mcb_status s;
+  if ((s = check_tensor(k, 4, 4)) || (s = check_tensor(v, 4, 4))) return s;
+  if (k->dtype != dtype || v->dtype != dtype) return MCB_STATUS_UNSUPPORTED_DTYPE;
+  for (int i = 0; i < 4; ++i)
+    if (k->dims[i] != v->dims[i]) return MCB_STATUS_SHAPE_MISMATCH;
+  if (k->dims[2] != kv_heads || k->dims[3] != dim) return MCB_STATUS_SHAPE_MISMATCH;
+  if (k->dims[1] < 1) return MCB_STATUS_INVALID_SHAPE;
+  if (k->dims[1] > 0x7fffffff || k->dims[0] > 0x7fffffff / k->dims[1])
+    return MCB_STATUS_INVALID_SHAPE;
+  return MCB_STATUS_OK;
+}
+
+mcb_status rope_impl(const mcb_tensor *q_out, const mcb_tensor *k_out, const mcb_tensor *v_cache,
+                     const mcb_tensor *q, const mcb_tensor *k, const mcb_tensor *v,
+                     const mcb_tensor *cos_sin, const mcb_tensor *positions,
+                     const mcb_tensor *slots, const uint8_t *axis_map, uint32_t flags, bool append,
+                     const mcb_exec *exec) {
+  mcb_status s;
+  if ((s = check_tensor(q, 3, 3)) || (s = check_tensor(k, 3, 3)) || (s = check_tensor(q_out, 3, 3)) ||
+      (s = check_tensor(cos_sin, 2, 2)) || (s = check_tensor(positions, 1, 2)))
+    return s;
+  if (!f_16_32(q->dtype) || k->dtype != q->dtype || q_out->dtype != q->dtype ||
+      cos_sin->dtype != MCB_DTYPE_F32 || positions->dtype != MCB_DTYPE_I32)
+    return MCB_STATUS_UNSUPPORTED_DTYPE;
+  const int64_t T = q->dims[0], H = q->dims[1], D = q->dims[2], HK = k->dims[1];
+  if (k->dims[0] != T || k->dims[2] != D) return MCB_STATUS_SHAPE_MISMATCH;
+  for (int i = 0; i < 3; ++i)
+    if (q_out->dims[i] != q->dims[i]) return MCB_STATUS_SHAPE_MISMATCH;
+  if (append) {
+    if ((s = check_tensor(v, 3, 3)) || (s = check_vector(slots, MCB_DTYPE_I32, T)) ||
+        (s = check_caches(k_out, v_cache, HK, D, q->dtype)))
+      return s;
+    if (v->dtype != q->dtype) return MCB_STATUS_UNSUPPORTED_DTYPE;
+    for (int i = 0; i < 3; ++i)
+      if (v->dims[i] != k->dims[i]) return MCB_STATUS_SHAPE_MISMATCH;
+  } else {
+    if ((s = check_tensor(k_out, 3, 3))) return s;
+    if (k_out->dtype != q->dtype) return MCB_STATUS_UNSUPPORTED_DTYPE;
+    for (int i = 0; i < 3; ++i)
+      if (k_out->dims[i] != k->dims[i]) return MCB_STATUS_SHAPE_MISMATCH;
+  }
+  const int64_t R = cos_sin->dims[1] / 2;
+  if (cos_sin->dims[1] % 2 != 0 || 2 * R > D || R > mcb::kMaxRopePairs || D > 0x7fffffff ||
+      H > 0x7fffffff || HK > 0x7fffffff)
+    return MCB_STATUS_INVALID_SHAPE;
+  const int64_t axes = positions->rank == 2 ? positions->dims[0] : 1;
+  if (positions->dims[positions->rank - 1] != T) return MCB_STATUS_SHAPE_MISMATCH;
+  if (axes < 1 || axes > 4) return MCB_STATUS_INVALID_SHAPE;
+  if (flags & ~(MCB_ROPE_PAIRED | MCB_ROPE_INVERSE)) return MCB_STATUS_INVALID_ARGUMENT;
+  if (axis_map)
+    for (int64_t i = 0; i < R; ++i)
+      if (axis_map[i] >= axes) return MCB_STATUS_INVALID_ARGUMENT;
+  if ((s = on_device({q_out, k_out, v_cache, q, k, v, cos_sin, positions, slots}))) return s;
+  if (T == 0 || D == 0) return MCB_STATUS_OK;
+  for (const mcb_tensor *o : {q_out, k_out, v_cache}) {
+    if (!o) continue;
+    for (const mcb_tensor *t : {q, k, v, cos_sin, positions, slots}) {
+      if (!t) continue;
+      if (((o == q_out && t == q) || (!append && o == k_out && t == k)) && same_place(o, t)) continue;
+      if (views_overlap(o, t)) return MCB_STATUS_ALIAS_VIOLATION;
+    }
+  }
+  if (views_overlap(q_out, k_out) || (append && (views_overlap(q_out, v_cache) ||
+                                                 overlaps(k_out, v_cache))))
+    return MCB_STATUS_ALIAS_VIOLATION;
+  Call call(exec);
+  if ((s = call.begin(false))) return s;
+  mcb::RopeParams p{};
+  p.q = q->data;
+  p.k = k->data;
+  p.q_out = q_out->data;
+  p.k_out = k_out->data;
+  p.cos_sin = f32(cos_sin);
+  p.positions = i32(positions);
+  p.tokens = T;
+  p.heads = static_cast<int32_t>(H);
+  p.kv_heads = static_cast<int32_t>(HK);
+  p.dim = static_cast<int32_t>(D);
+  p.pairs = static_cast<int32_t>(R);
+  for (int i = 0; i < 2; ++i) {
+    p.q_s[i] = q->strides[i];
+    p.k_s[i] = k->strides[i];
+    p.qo_s[i] = q_out->strides[i];
+    p.v_s[i] = append ? v->strides[i] : 0;
+  }
+  for (int i = 0; i < 3; ++i) {
+    p.ko_s[i] = k_out->strides[i];
+    p.vo_s[i] = append ? v_cache->strides[i] : 0;
+  }
+  if (append) {
+    p.v = v->data;
+    p.v_out = v_cache->data;
+    p.slots = i32(slots);
+    p.block = static_cast<int32_t>(k_out->dims[1]);
+    p.cache_slots = k_out->dims[0] * k_out->dims[1];
+  }
+  p.pos_stride = positions->rank == 2 ? positions->strides[0] : 0;
+  p.table_stride = cos_sin->strides[0];
+  p.table_rows = cos_sin->dims[0];
+  p.paired = (flags & MCB_ROPE_PAIRED) != 0;
+  p.inverse = (flags & MCB_ROPE_INVERSE) != 0;
+  if (axis_map) std::memcpy(p.axis, axis_map, static_cast<size_t>(R));
+  LaunchInfo info;
+  call.mark_compute_start();
+  const cudaError_t err =
+      mcb::launch_rope(p, static_cast<int>(q->dtype), call.sms(), call.stream(), &info);
+  call.mark_compute_end();
+  return call.finish(nullptr, nullptr, info, err);
+}
+
+mcb_status tree_attention_impl(const mcb_tensor *o, const mcb_tensor *lse, const mcb_tensor *q,
+                               const mcb_tensor *k, const mcb_tensor *v, const mcb_tensor *table,
+                               const mcb_tensor *cu, const mcb_tensor *kv_lens,
+                               const mcb_tensor *mask, double scale, const mcb_exec *exec) {
+  mcb_status s;
+  if ((s = check_tensor(q, 3, 3)) || (s = check_tensor(o, 3, 3)) || (s = check_tensor(table, 2, 2)))
+    return s;
+  if (!f_16_32(q->dtype) || o->dtype != q->dtype || table->dtype != MCB_DTYPE_I32)
+    return MCB_STATUS_UNSUPPORTED_DTYPE;
+  const int64_t T = q->dims[0], H = q->dims[1], D = q->dims[2], B = table->dims[0];
+  for (int i = 0; i < 3; ++i)
+    if (o->dims[i] != q->dims[i]) return MCB_STATUS_SHAPE_MISMATCH;
+  if ((s = check_tensor(k, 4, 4))) return s;
+  const int64_t HK = k->dims[2];
+  if ((s = check_caches(k, v, HK, D, q->dtype)) || (s = check_vector(cu, MCB_DTYPE_I32, B + 1)) ||
+      (s = check_vector(kv_lens, MCB_DTYPE_I32, B)))
+    return s;
+  if (H > 65535 || HK < 1 || H % HK != 0 || D < 1 || B > 0x7fffffff || T > 0x7fffffff ||
+      table->dims[1] > 0x7fffffff)
+    return MCB_STATUS_INVALID_SHAPE;
+  if (mask) {
+    if ((s = check_tensor(mask, 2, 2))) return s;
+    if (mask->dtype != MCB_DTYPE_I32) return MCB_STATUS_UNSUPPORTED_DTYPE;
+    if (mask->dims[0] != T) return MCB_STATUS_SHAPE_MISMATCH;
+  }
+  if (lse) {
+    if ((s = check_tensor(lse, 2, 2))) return s;
+    if (lse->dtype != MCB_DTYPE_F32) return MCB_STATUS_UNSUPPORTED_DTYPE;
+    if (lse->dims[0] != T || lse->dims[1] != H) return MCB_STATUS_SHAPE_MISMATCH;
+  }
+  if (!std::isfinite(static_cast<float>(scale))) return MCB_STATUS_INVALID_ARGUMENT;
+  if ((s = on_device({o, lse, q, k, v, table, cu, kv_lens, mask}))) return s;
+  for (const mcb_tensor *out : {o, lse})
+    for (const mcb_tensor *t : {q, k, v, table, cu, kv_lens, mask})
+      if (overlaps(out, t)) return MCB_STATUS_ALIAS_VIOLATION;
+  if (overlaps(o, lse)) return MCB_STATUS_ALIAS_VIOLATION;
+  if (T == 0 || H == 0) return MCB_STATUS_OK;
+  Call call(exec);
+  if ((s = call.begin(false))) return s;
+  mcb::TreeAttn p{};
+  p.q = q->data;
+  p.k = k->data;
+  p.v = v->data;
+  p.o = o->data;
+  p.lse = lse ? static_cast<float *>(lse->data) : nullptr;
+  p.table = i32(table);
+  p.cu = i32(cu);
+  p.kv_lens = i32(kv_lens);
+  p.mask = mask ? static_cast<const uint32_t *>(mask->data) : nullptr;
+  p.tokens = T;
+  p.requests = B;
+  p.heads = static_cast<int32_t>(H);
+  p.kv_heads = static_cast<int32_t>(HK);
+  p.dim = static_cast<int32_t>(D);
+  p.block = static_cast<int32_t>(k->dims[1]);
+  for (int i = 0; i < 2; ++i) {
+    p.q_s[i] = q->strides[i];
+    p.o_s[i] = o->strides[i];
+  }
+  p.lse_s = lse ? lse->strides[0] : 0;
+  for (int i = 0; i < 3; ++i) {
+    p.k_s[i] = k->strides[i];
+    p.v_s[i] = v->strides[i];
+  }
+  p.columns = table->dims[1];
+  p.table_stride = table->strides[0];
+  p.blocks = k->dims[0];
+  p.mask_words = mask ? mask->dims[1] : 0;
+  p.mask_stride = mask ? mask->strides[0] : 0;
+  p.scale = static_cast<float>(scale);
+  LaunchInfo info;
+  void *scratch = nullptr;
+  const uint64_t bytes = mcb::tree_attn_simt_scratch(p, call.sms());
+  if (bytes && (s = call.scratch(bytes, &scratch))) return s;
+  call.mark_compute_start();
+  const cudaError_t err =
+      mcb::launch_tree_attn_simt(p, static_cast<int>(q->dtype), static_cast<float *>(scratch),
+                                 call.sms(), call.stream(), &info);
+  call.mark_compute_end();
+  if (err == cudaErrorNotSupported) return MCB_STATUS_UNAVAILABLE_VARIANT;
+  return call.finish(nullptr, nullptr, info, err);
+}
+
+mcb_status adjust_logits_impl(const mcb_tensor *out, const mcb_tensor *x, const mcb_tensor *ids,
+                              const mcb_tensor *cu, const mcb_tensor *prompt_lens,
+                              const mcb_tensor *repetition, const mcb_tensor *presence,
+                              const mcb_tensor *frequency, const mcb_tensor *bias_ids,
+                              const mcb_tensor *bias_values, const mcb_tensor *bias_cu,
+                              const mcb_tensor *allowed, const mcb_exec *exec) {
+  mcb_status s;
+  if ((s = check_tensor(x, 2, 2)) || (s = check_tensor(out, 2, 2))) return s;
+  if (!f_16_32(x->dtype) || (out->dtype != x->dtype && out->dtype != MCB_DTYPE_F32))
+    return MCB_STATUS_UNSUPPORTED_DTYPE;
+  const int64_t R = x->dims[0], V = x->dims[1];
+  if (out->dims[0] != R || out->dims[1] != V) return MCB_STATUS_SHAPE_MISMATCH;
+  if ((s = check_vector(ids, MCB_DTYPE_I32, -1)) || (s = check_vector(cu, MCB_DTYPE_I32, R + 1)) ||
+      (s = check_vector(prompt_lens, MCB_DTYPE_I32, R)))
+    return s;
+  for (const mcb_tensor *t : {repetition, presence, frequency})
+    if (t && (s = check_vector(t, MCB_DTYPE_F32, R))) return s;
+  if (!bias_ids != !bias_values || !bias_ids != !bias_cu) return MCB_STATUS_INVALID_ARGUMENT;
+  if (bias_ids && ((s = check_vector(bias_ids, MCB_DTYPE_I32, -1)) ||
+                   (s = check_vector(bias_values, MCB_DTYPE_F32, bias_ids->dims[0])) ||
+                   (s = check_vector(bias_cu, MCB_DTYPE_I32, R + 1))))
+    return s;
+  if (allowed) {
+    if ((s = check_tensor(allowed, 2, 2))) return s;
+    if (allowed->dtype != MCB_DTYPE_I32) return MCB_STATUS_UNSUPPORTED_DTYPE;
+    if (allowed->dims[0] != R || allowed->dims[1] != (V + 31) / 32) return MCB_STATUS_SHAPE_MISMATCH;
+  }
+  if (V > 0x7fffffff || ids->dims[0] > 0x7fffffff || (bias_ids && bias_ids->dims[0] > 0x7fffffff))
+    return MCB_STATUS_INVALID_SHAPE;
+  if ((s = on_device({out, x, ids, cu, prompt_lens, repetition, presence, frequency, bias_ids,
+                      bias_values, bias_cu, allowed})))
+    return s;
+  if (overlaps(out, x) && !same_place(out, x)) return MCB_STATUS_ALIAS_VIOLATION;
+  for (const mcb_tensor *t : {ids, cu, prompt_lens, repetition, presence, frequency, bias_ids,
+                              bias_values, bias_cu, allowed})
+    if (overlaps(out, t)) return MCB_STATUS_ALIAS_VIOLATION;
+  if (R == 0 || V == 0) return MCB_STATUS_OK;
+  Call call(exec);
+  if ((s = call.begin(false))) return s;
+  mcb::LogitsParams p{};
+  p.logits = x->data;
+  p.out = out->data;
+  p.token_ids = i32(ids);
+  p.cu = i32(cu);
+  p.prompt_lens = i32(prompt_lens);
+  p.repetition = f32(repetition);
+  p.presence = f32(presence);
+  p.frequency = f32(frequency);
+  p.bias_ids = i32(bias_ids);
+  p.bias_values = f32(bias_values);
+  p.bias_cu = i32(bias_cu);
+  p.allowed = allowed ? static_cast<const uint32_t *>(allowed->data) : nullptr;
+  p.rows = R;
+  p.vocab = V;
+  p.ld_in = x->strides[0];
+  p.ld_out = out->strides[0];
+  p.ld_mask = allowed ? allowed->strides[0] : 0;
+  p.tokens = ids->dims[0];
+  p.biases = bias_ids ? bias_ids->dims[0] : 0;
+  LaunchInfo info;
+  call.mark_compute_start();
+  const cudaError_t err = mcb::launch_logits(p, static_cast<int>(x->dtype),
+                                             static_cast<int>(out->dtype), call.stream(), &info);
+  call.mark_compute_end();
+  if (err == cudaErrorNotSupported) return MCB_STATUS_UNAVAILABLE_VARIANT;
+  return call.finish(nullptr, nullptr, info, err);
+}
+
 }  // namespace
 
 // =====================================================================================
@@ -2510,6 +2920,88 @@ MCB_API mcb_status mcb_device_zero_raw_on_stream(void *device_ptr, uint64_t size
   if (size_bytes && !device_ptr) return MCB_STATUS_INVALID_ARGUMENT;
   return from_cuda(
       cudaMemsetAsync(device_ptr, 0, size_bytes, static_cast<cudaStream_t>(stream)));
+}
+
+MCB_API mcb_status mcb_paged_grow_v1(const mcb_tensor *block_table, const mcb_tensor *slots,
+                                     const mcb_tensor *positions, const mcb_tensor *cu_new,
+                                     const mcb_tensor *len_after, const mcb_tensor *free_left,
+                                     const mcb_tensor *lens, const mcb_tensor *new_lens,
+                                     const mcb_tensor *free_blocks, const mcb_tensor *free_count,
+                                     int64_t block, const mcb_exec *exec) noexcept {
+  try {
+    return paged_grow_impl(block_table, slots, positions, cu_new, len_after, free_left, lens,
+                           new_lens, free_blocks, free_count, block, exec);
+  } catch (...) {
+    return MCB_STATUS_CANDIDATE_FAILURE;
+  }
+}
+
+MCB_API mcb_status mcb_paged_release_v1(const mcb_tensor *free_blocks, const mcb_tensor *free_left,
+                                        const mcb_tensor *block_table, const mcb_tensor *lens,
+                                        const mcb_tensor *keep_lens, const mcb_tensor *free_count,
+                                        int64_t block, const mcb_exec *exec) noexcept {
+  try {
+    return paged_release_impl(free_blocks, free_left, block_table, lens, keep_lens, free_count,
+                              block, exec);
+  } catch (...) {
+    return MCB_STATUS_CANDIDATE_FAILURE;
+  }
+}
+
+MCB_API mcb_status mcb_rope_v1(const mcb_tensor *q_out, const mcb_tensor *k_out,
+                               const mcb_tensor *q, const mcb_tensor *k,
+                               const mcb_tensor *cos_sin, const mcb_tensor *positions,
+                               const uint8_t *axis_map, uint32_t flags,
+                               const mcb_exec *exec) noexcept {
+  try {
+    return rope_impl(q_out, k_out, nullptr, q, k, nullptr, cos_sin, positions, nullptr, axis_map,
+                     flags, false, exec);
+  } catch (...) {
+    return MCB_STATUS_CANDIDATE_FAILURE;
+  }
+}
+
+MCB_API mcb_status mcb_rope_append_v1(const mcb_tensor *q_out, const mcb_tensor *k_cache,
+                                      const mcb_tensor *v_cache, const mcb_tensor *q,
+                                      const mcb_tensor *k, const mcb_tensor *v,
+                                      const mcb_tensor *cos_sin, const mcb_tensor *positions,
+                                      const mcb_tensor *slots, const uint8_t *axis_map,
+                                      uint32_t flags, const mcb_exec *exec) noexcept {
+  try {
+    return rope_impl(q_out, k_cache, v_cache, q, k, v, cos_sin, positions, slots, axis_map, flags,
+                     true, exec);
+  } catch (...) {
+    return MCB_STATUS_CANDIDATE_FAILURE;
+  }
+}
+
+MCB_API mcb_status mcb_tree_attention_v1(const mcb_tensor *o, const mcb_tensor *lse,
+                                         const mcb_tensor *q, const mcb_tensor *k_cache,
+                                         const mcb_tensor *v_cache, const mcb_tensor *block_table,
+                                         const mcb_tensor *cu_new, const mcb_tensor *kv_lens,
+                                         const mcb_tensor *tree_mask, double scale,
+                                         const mcb_exec *exec) noexcept {
+  try {
+    return tree_attention_impl(o, lse, q, k_cache, v_cache, block_table, cu_new, kv_lens, tree_mask,
+                               scale, exec);
+  } catch (...) {
+    return MCB_STATUS_CANDIDATE_FAILURE;
+  }
+}
+
+MCB_API mcb_status mcb_adjust_logits_v1(const mcb_tensor *out, const mcb_tensor *logits,
+                                        const mcb_tensor *token_ids, const mcb_tensor *cu_tokens,
+                                        const mcb_tensor *prompt_lens,
+                                        const mcb_tensor *repetition, const mcb_tensor *presence,
+                                        const mcb_tensor *frequency, const mcb_tensor *bias_ids,
+                                        const mcb_tensor *bias_values, const mcb_tensor *bias_cu,
+                                        const mcb_tensor *allowed, const mcb_exec *exec) noexcept {
+  try {
+    return adjust_logits_impl(out, logits, token_ids, cu_tokens, prompt_lens, repetition, presence,
+                              frequency, bias_ids, bias_values, bias_cu, allowed, exec);
+  } catch (...) {
+    return MCB_STATUS_CANDIDATE_FAILURE;
+  }
 }
 
 }  // extern "C"

@@ -247,6 +247,74 @@ cudaError_t launch_peer_wait(const uint32_t *flag, uint32_t target, long long li
 // then stores `value` to `flag` (the peer's memory) with release semantics.
 cudaError_t launch_peer_signal(uint32_t *flag, uint32_t value, cudaStream_t stream);
 
+// ---- paged.cu: block tables and slot maps of a paged cache ------------------------------------
+struct PagedGrow {
+  int32_t *table, *slots, *positions, *cu, *after, *free_left;
+  const int32_t *lens, *new_lens, *free, *free_count;
+  int64_t requests, columns, table_stride, tokens, free_capacity;
+  int32_t block;
+};
+cudaError_t launch_paged_grow(const PagedGrow &p, cudaStream_t stream, LaunchInfo *info);
+struct PagedRelease {
+  int32_t *free, *free_left;
+  const int32_t *table, *lens, *keep_lens, *free_count;
+  int64_t requests, columns, table_stride, free_capacity;
+  int32_t block;
+};
+cudaError_t launch_paged_release(const PagedRelease &p, cudaStream_t stream, LaunchInfo *info);
+
+// ---- rope.cu: rotary positions, and the append to a paged cache -----------------------------
+constexpr int kMaxRopePairs = 128;
+struct RopeParams {
+  const void *q, *k, *v;  // v only when appending
+  void *q_out, *k_out, *v_out;
+  const float *cos_sin;
+  const int32_t *positions, *slots;  // slots: k_out and v_out are caches
+  int64_t tokens;
+  int32_t heads, kv_heads, dim, pairs;
+  int64_t q_s[2], k_s[2], v_s[2], qo_s[2];  // [token, head] element strides
+  int64_t ko_s[3], vo_s[3];  // [token, head], or of a cache [block, row, head]
+  int64_t pos_stride, table_stride, table_rows, cache_slots;
+  int32_t block, paired, inverse;
+  uint8_t axis[kMaxRopePairs];  // position row of each pair
+};
+cudaError_t launch_rope(const RopeParams &p, int dtype, int sms, cudaStream_t stream,
+                        LaunchInfo *info);
+
+// ---- tree_attn.cu: attention of drafted tokens over a paged cache ------------------------------
+struct TreeAttn {
+  const void *q, *k, *v;
+  void *o;
+  float *lse;  // or nullptr
+  const int32_t *table, *cu, *kv_lens;
+  const uint32_t *mask;  // or nullptr: causal
+  int64_t tokens, requests;
+  int32_t heads, kv_heads, dim, block;
+  int64_t q_s[2], o_s[2], lse_s;         // [token, head]
+  int64_t k_s[3], v_s[3];                // [block, row, head]
+  int64_t columns, table_stride, blocks; // block table row; blocks of the cache
+  int64_t mask_words, mask_stride;
+  float scale;
+};
+// Bytes of device scratch that launch_tree_attn_simt needs for its partial results.
+uint64_t tree_attn_simt_scratch(const TreeAttn &p, int sms);
+cudaError_t launch_tree_attn_simt(const TreeAttn &p, int dtype, float *scratch, int sms,
+                                  cudaStream_t stream, LaunchInfo *info);
+
+// ---- logits.cu: penalties, biases and grammar masks ---------------------------------------------
+struct LogitsParams {
+  const void *logits;
+  void *out;
+  const int32_t *token_ids, *cu, *prompt_lens;
+  const float *repetition, *presence, *frequency;  // or nullptr
+  const int32_t *bias_ids, *bias_cu;               // or nullptr
+  const float *bias_values;
+  const uint32_t *allowed;  // or nullptr
+  int64_t rows, vocab, ld_in, ld_out, ld_mask, tokens, biases;
+};
+cudaError_t launch_logits(const LogitsParams &p, int in_dtype, int out_dtype, cudaStream_t stream,
+                          LaunchInfo *info);
+
 // Tensor-map encoder (driver entry point fetched once through the runtime).
 bool encode_tmap_2d(CUtensorMap *map, CUtensorMapDataType dtype, const void *base,
                     uint64_t inner, uint64_t outer, uint64_t row_stride_bytes, uint32_t box_inner,

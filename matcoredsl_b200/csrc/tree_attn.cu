@@ -1,0 +1,304 @@
+// Attention of a tree of drafted tokens over a paged key/value cache, on CUDA
+// cores: any element type, head size up to 256, strides and alignment.
+//
+// Request b's new tokens i = 0 .. n-1 sit at the end of its kv_len keys, token
+// i at position P + i with P = kv_len - n. Row i sees every key before P, and
+// of the new ones those whose bit is set in its mask row (without a mask:
+// j <= i). o = sum_j p_j v_j / l, p_j = exp(scale q.k_j - m), l = sum_j p_j,
+// lse = m + log l; a row that sees nothing gives o = 0, lse = -inf.
+//
+// One CTA (4 warps) per token, key head, group of kRows query heads and slice
+// of the keys. A warp takes 32 keys at a time: each lane computes kRows dot
+// products with its own key, the softmax runs across the lanes with one running
+// maximum and sum a row, then the lanes turn to the value rows, one element
+// slice each. Keys that the token does not see are skipped, never multiplied by
+// zero, so infinities and NaN in their values do not reach it.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "internal.h"
+
+namespace mcb {
+namespace {
+
+constexpr int WARPS = 4;
+constexpr int THREADS = WARPS * 32;
+constexpr int MAX_SPLITS = 64;
+constexpr int MIN_KEYS = 256;  // keys a slice is worth a CTA for
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v) {
+  return static_cast<float>(v);
+}
+
+// Number of the request that token t belongs to, -1 when it belongs to none.
+__device__ __forceinline__ int32_t request_of(const TreeAttn &p, int64_t t) {
+  int64_t lo = 0, hi = p.requests;  // the last b with cu[b] <= t
+  while (hi - lo > 1) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (p.cu[mid] <= t)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  if (p.requests == 0 || t < p.cu[lo] || t >= p.cu[lo + 1]) return -1;
+  return static_cast<int32_t>(lo);
+}
+
+// kRows query heads of one token; kCols = elements of a head per lane.
+template <typename T, int kRows, int kCols>
+__global__ void __launch_bounds__(THREADS) tree_attn_simt_kernel(const TreeAttn p, float *partial,
+                                                                 int splits) {
+  extern __shared__ float smem[];
+  float *qs = smem;                                     // [kRows][dim]
+  float *red = smem + kRows * p.dim;                    // [WARPS][kRows][dim + 2]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int group = p.heads / p.kv_heads;
+  const int groups = (group + kRows - 1) / kRows;
+  const int64_t t = blockIdx.x;
+  const int hk = blockIdx.y / groups, g0 = (blockIdx.y - hk * groups) * kRows;
+  const int rows = min(kRows, group - g0);
+  const int h0 = hk * group + g0;  // first query head
+  const T *q = static_cast<const T *>(p.q) + t * p.q_s[0] + h0 * p.q_s[1];
+  for (int i = threadIdx.x; i < kRows * p.dim; i += THREADS) {
+    const int r = i / p.dim, d = i - r * p.dim;
+    qs[i] = r < rows ? to_f32(q[r * p.q_s[1] + d]) * p.scale : 0.0f;
+  }
+  __syncthreads();
+  float m[kRows], l[kRows], acc[kRows][kCols];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) acc[r][c] = 0.0f;
+  }
+  const int32_t b = request_of(p, t);
+  if (b >= 0) {
+    const int64_t i = t - p.cu[b], n = p.cu[b + 1] - p.cu[b];
+    const int64_t kv = max(0, p.kv_lens[b]), prefix = kv - n;
+    const int64_t keys = min(kv, p.columns * p.block);
+    const int64_t per = ((keys + splits - 1) / splits + 31) / 32 * 32;
+    const int64_t first = per * blockIdx.z, last = min(keys, first + per);
+    for (int64_t k0 = first + warp * 32; k0 < last; k0 += WARPS * 32) {
+      const int64_t pos = k0 + lane;
+      bool visible = pos < last;
+      int64_t ko = 0, vo = 0;
+      if (visible) {
+        const int64_t col = pos / p.block, off = pos - col * p.block;
+        const int32_t blk = p.table[b * p.table_stride + col];
+        visible = blk >= 0 && blk < p.blocks;
+        const int64_t j = pos - prefix;
+        if (visible && j >= 0)
+          visible = p.mask ? (j >> 5) < p.mask_words &&
+                                 ((p.mask[t * p.mask_stride + (j >> 5)] >> (j & 31)) & 1u)
+                           : j <= i;
+        ko = blk * p.k_s[0] + off * p.k_s[1] + hk * p.k_s[2];
+        vo = blk * p.v_s[0] + off * p.v_s[1] + hk * p.v_s[2];
+      }
+      const uint32_t seen = __ballot_sync(0xffffffffu, visible);
+      if (seen == 0) continue;
+      float s[kRows];
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) s[r] = 0.0f;
+      if (visible) {
+        const T *k = static_cast<const T *>(p.k) + ko;
+        for (int d = 0; d < p.dim; ++d) {
+          const float x = to_f32(k[d]);
+#pragma unroll
+          for (int r = 0; r < kRows; ++r) s[r] = fmaf(qs[r * p.dim + d], x, s[r]);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        if (!visible) s[r] = -INFINITY;
+        float mx = s[r];
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        mx = fmaxf(mx, m[r]);
+        // A row whose scores are all -inf (or NaN) so far: keep exponents defined.
+        const float ref = mx == -INFINITY ? 0.0f : mx;
+        const float f = expf(m[r] - ref);
+        s[r] = visible ? expf(s[r] - ref) : 0.0f;
+        float sum = s[r];
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        l[r] = l[r] * f + sum;
+        m[r] = mx;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) acc[r][c] *= f;
+      }
+      for (uint32_t left = seen; left; left &= left - 1) {
+        const int j = __ffs(left) - 1;
+        const T *v = static_cast<const T *>(p.v) + __shfl_sync(0xffffffffu, vo, j);
+        float w[kRows];
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) w[r] = __shfl_sync(0xffffffffu, s[r], j);
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+          const int d = c * 32 + lane;
+          const float x = d < p.dim ? to_f32(v[d]) : 0.0f;
+#pragma unroll
+          for (int r = 0; r < kRows; ++r) acc[r][c] = fmaf(w[r], x, acc[r][c]);
+        }
+      }
+    }
+  }
+  // Join the warps, in their order.
+  const int stride = p.dim + 2;
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    float *out = red + (warp * kRows + r) * stride;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+      if (c * 32 + lane < p.dim) out[c * 32 + lane] = acc[r][c];
+    if (lane == 0) {
+      out[p.dim] = m[r];
+      out[p.dim + 1] = l[r];
+    }
+  }
+  __syncthreads();
+  for (int r = warp; r < rows; r += WARPS) {
+    float mx = -INFINITY;
+    for (int w = 0; w < WARPS; ++w) mx = fmaxf(mx, red[(w * kRows + r) * stride + p.dim]);
+    const float ref = mx == -INFINITY ? 0.0f : mx;
+    float f[WARPS], sum = 0.0f;
+    for (int w = 0; w < WARPS; ++w) {
+      const float *in = red + (w * kRows + r) * stride;
+      f[w] = expf(in[p.dim] - ref);
+      sum += in[p.dim + 1] * f[w];
+    }
+    const int64_t row = t * p.heads + h0 + r;
+    float *part = partial ? partial + (row * splits + blockIdx.z) * stride : nullptr;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T *o = static_cast<T *>(p.o) + t * p.o_s[0] + (h0 + r) * p.o_s[1];
+    for (int d = lane; d < p.dim; d += 32) {
+      float x = 0.0f;
+      for (int w = 0; w < WARPS; ++w) {
+        const float *in = red + (w * kRows + r) * stride;
+        if (in[p.dim + 1] != 0.0f) x = fmaf(in[d], f[w], x);
+      }
+      if (part)
+        part[d] = x;
+      else
+        o[d] = static_cast<T>(x * inv);
+    }
+    if (lane == 0) {
+      if (part) {
+        part[p.dim] = mx;
+        part[p.dim + 1] = sum;
+      } else if (p.lse) {
+        p.lse[t * p.lse_s + h0 + r] = sum == 0.0f ? -INFINITY : ref + logf(sum);
+      }
+    }
+  }
+}
+
+// Joins the key slices of a row, in their order: one warp a row.
+template <typename T>
+__global__ void __launch_bounds__(256) tree_attn_join_kernel(const TreeAttn p, const float *partial,
+                                                             int splits) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= p.tokens * p.heads) return;
+  const int64_t t = row / p.heads, h = row - t * p.heads;
+  const int stride = p.dim + 2;
+  const float *in = partial + row * splits * stride;
+  float mx = -INFINITY, sum = 0.0f;
+  for (int z = 0; z < splits; ++z) mx = fmaxf(mx, in[z * stride + p.dim]);
+  const float ref = mx == -INFINITY ? 0.0f : mx;
+  for (int z = 0; z < splits; ++z)
+    sum += in[z * stride + p.dim + 1] * expf(in[z * stride + p.dim] - ref);
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  T *o = static_cast<T *>(p.o) + t * p.o_s[0] + h * p.o_s[1];
+  for (int d = lane; d < p.dim; d += 32) {
+    float x = 0.0f;
+    for (int z = 0; z < splits; ++z)
+      if (in[z * stride + p.dim + 1] != 0.0f)
+        x = fmaf(in[z * stride + d], expf(in[z * stride + p.dim] - ref), x);
+    o[d] = static_cast<T>(x * inv);
+  }
+  if (lane == 0 && p.lse)
+    p.lse[t * p.lse_s + h] = sum == 0.0f ? -INFINITY : ref + logf(sum);
+}
+
+int rows_of(const TreeAttn &p) {
+  const int group = p.heads / p.kv_heads;
+  return group == 1 ? 1 : group <= 4 ? 4 : 8;
+}
+
+int splits_of(const TreeAttn &p, int sms) {
+  const int group = p.heads / p.kv_heads, r = rows_of(p);
+  const int64_t units = p.tokens * p.kv_heads * ((group + r - 1) / r);
+  int64_t s = units > 0 ? 8 * sms / units : 1;
+  const int64_t most = p.columns * p.block / MIN_KEYS;
+  s = s < most ? s : most;
+  s = s < MAX_SPLITS ? s : MAX_SPLITS;
+  return s < 1 ? 1 : static_cast<int>(s);
+}
+
+template <typename T, int kRows, int kCols>
+cudaError_t run(const TreeAttn &p, float *scratch, int splits, cudaStream_t stream) {
+  const int group = p.heads / p.kv_heads;
+  const dim3 grid(static_cast<unsigned>(p.tokens),
+                  static_cast<unsigned>(p.kv_heads * ((group + kRows - 1) / kRows)),
+                  static_cast<unsigned>(splits));
+  const size_t smem = sizeof(float) * (kRows * p.dim + WARPS * kRows * (p.dim + 2));
+  static_assert(sizeof(float) * (8 * 256 + WARPS * 8 * 258) <= 48 * 1024, "no opt-in needed");
+  tree_attn_simt_kernel<T, kRows, kCols><<<grid, THREADS, smem, stream>>>(
+      p, splits > 1 ? scratch : nullptr, splits);
+  if (splits > 1)
+    tree_attn_join_kernel<T><<<static_cast<unsigned>((p.tokens * p.heads + 7) / 8), 256, 0,
+                               stream>>>(p, scratch, splits);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t run_type(const TreeAttn &p, float *scratch, int splits, cudaStream_t stream) {
+  const int r = rows_of(p);
+  auto cols = [&](auto rows) {
+    constexpr int R = decltype(rows)::value;
+    return p.dim <= 64    ? run<T, R, 2>(p, scratch, splits, stream)
+           : p.dim <= 128 ? run<T, R, 4>(p, scratch, splits, stream)
+                          : run<T, R, 8>(p, scratch, splits, stream);
+  };
+  if (r == 1) return cols(std::integral_constant<int, 1>{});
+  if (r == 4) return cols(std::integral_constant<int, 4>{});
+  return cols(std::integral_constant<int, 8>{});
+}
+
+}  // namespace
+
+uint64_t tree_attn_simt_scratch(const TreeAttn &p, int sms) {
+  const int splits = splits_of(p, sms);
+  if (splits == 1) return 0;
+  return static_cast<uint64_t>(p.tokens) * p.heads * splits * (p.dim + 2) * sizeof(float);
+}
+
+cudaError_t launch_tree_attn_simt(const TreeAttn &p, int dtype, float *scratch, int sms,
+                                  cudaStream_t stream, LaunchInfo *info) {
+  const int group = p.heads / p.kv_heads, r = rows_of(p);
+  const int64_t gy = static_cast<int64_t>(p.kv_heads) * ((group + r - 1) / r);
+  if (p.dim > 256 || p.tokens > 0x7fffffff || gy > 65535 ||
+      (p.tokens * p.heads + 7) / 8 > 0x7fffffff)
+    return cudaErrorNotSupported;
+  const int splits = splits_of(p, sms);
+  cudaError_t e;
+  if (dtype == MCB_DTYPE_F32)
+    e = run_type<float>(p, scratch, splits, stream);
+  else if (dtype == MCB_DTYPE_F16)
+    e = run_type<__half>(p, scratch, splits, stream);
+  else
+    e = run_type<__nv_bfloat16>(p, scratch, splits, stream);
+  info->launches = splits > 1 ? 2 : 1;
+  info->tile_m = r;
+  info->tile_n = 32;
+  info->ctas = static_cast<int>(p.tokens * gy * splits);
+  info->set_route("simt_tree_attention");
+  return e;
+}
+
+}  // namespace mcb
