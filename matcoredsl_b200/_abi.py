@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmcb.so")
@@ -244,7 +245,41 @@ def load() -> ctypes.CDLL:
     return lib
 
 
-_TENSOR_SIZE = ctypes.sizeof(Tensor)
+_TENSOR_SIZE = TENSOR_SIZE = ctypes.sizeof(Tensor)
+EXEC_SIZE, REPORT_SIZE = ctypes.sizeof(Exec), ctypes.sizeof(Report)
+
+# Packers of whole structures, in native alignment like the ctypes mirrors
+# above (x: zero bytes): a tensor of rank r takes (abi_version, struct_size,
+# data, dtype, rank, r dims, r strides, memory_space), an execution context
+# (abi_version, struct_size, device, flags, stream, workspace, workspace_bytes,
+# report), a report its first two fields.
+TENSOR_PACK = [struct.Struct(f"@IIQII{r}q{8 * (MAX_RANK - r)}x{r}q{8 * (MAX_RANK - r)}xI20x").pack_into
+               for r in range(MAX_RANK + 1)]
+EXEC_PACK = struct.Struct("@IIiIQQQQ16x").pack_into
+REPORT_PACK = struct.Struct(f"@II{REPORT_SIZE - 8}x").pack_into
+
+_frames = {}  # (entry point, operands) -> what call_frame returns, buffers aside
+
+
+def call_frame(fn_name: str, operands: int):
+    """(fn, buffer, its address, offset of the exec, offset of the report) for
+    one call of an entry point whose first arguments are `operands` tensor
+    descriptors. fn takes addresses (None: no operand); the buffer is a new
+    one each time, so calls from several threads do not share it."""
+    got = _frames.get((fn_name, operands))
+    if got is None:
+        lib = load()
+        fn = lib[fn_name]  # a function object of its own, next to the declared one
+        res, args = SIGNATURES[fn_name]
+        fn.restype = res
+        fn.argtypes = [ctypes.c_void_p if i < operands or i == len(args) - 1 else a
+                       for i, a in enumerate(args)]
+        size = operands * TENSOR_SIZE + EXEC_SIZE + REPORT_SIZE
+        got = _frames[fn_name, operands] = (fn, ctypes.c_char * size, operands * TENSOR_SIZE)
+    fn, buffer, ex = got
+    buf = buffer()
+    return fn, buf, ctypes.addressof(buf), ex, ex + EXEC_SIZE
+
 
 
 def make_tensor(ptr: int, dtype: str, shape, strides, device: bool) -> Tensor:
