@@ -46,6 +46,7 @@ SOURCES = {
     "paged.cu": [],
     "rope.cu": [],
     "tree_attn.cu": [],
+    "tree_attn_tc.cu": [],
     "logits.cu": [],
 }
 HEADERS = ["common.cuh", "internal.h", "epilogue.cuh"]

@@ -2274,12 +2274,17 @@ mcb_status tree_attention_impl(const mcb_tensor *o, const mcb_tensor *lse, const
   p.scale = static_cast<float>(scale);
   LaunchInfo info;
   void *scratch = nullptr;
-  const uint64_t bytes = mcb::tree_attn_simt_scratch(p, call.sms());
+  const int dt = static_cast<int>(q->dtype);
+  const bool tc = mcb::tree_attn_tc_ok(p, dt);
+  const uint64_t bytes = tc ? mcb::tree_attn_tc_scratch(p, call.sms())
+                            : mcb::tree_attn_simt_scratch(p, call.sms());
   if (bytes && (s = call.scratch(bytes, &scratch))) return s;
   call.mark_compute_start();
   const cudaError_t err =
-      mcb::launch_tree_attn_simt(p, static_cast<int>(q->dtype), static_cast<float *>(scratch),
-                                 call.sms(), call.stream(), &info);
+      tc ? mcb::launch_tree_attn_tc(p, dt, scratch, call.ctx()->status, call.sms(), call.stream(),
+                                    &info)
+         : mcb::launch_tree_attn_simt(p, dt, static_cast<float *>(scratch), call.sms(),
+                                      call.stream(), &info);
   call.mark_compute_end();
   if (err == cudaErrorNotSupported) return MCB_STATUS_UNAVAILABLE_VARIANT;
   return call.finish(nullptr, nullptr, info, err);

@@ -301,6 +301,17 @@ uint64_t tree_attn_simt_scratch(const TreeAttn &p, int sms);
 cudaError_t launch_tree_attn_simt(const TreeAttn &p, int dtype, float *scratch, int sms,
                                   cudaStream_t stream, LaunchInfo *info);
 
+// ---- tree_attn_tc.cu: the same on tcgen05 ------------------------------------------------------
+// A unit of rows whose key tiles lie in several CTAs (left by the first of them).
+struct TreeAttnPart {
+  int32_t parts;  // CTAs it lies in, 0: no such unit starts in this CTA
+  int32_t tok0, head, row0, nrows;
+};
+bool tree_attn_tc_ok(const TreeAttn &p, int dtype);
+uint64_t tree_attn_tc_scratch(const TreeAttn &p, int sms);
+cudaError_t launch_tree_attn_tc(const TreeAttn &p, int dtype, void *scratch, uint32_t *status,
+                                int sms, cudaStream_t stream, LaunchInfo *info);
+
 // ---- logits.cu: penalties, biases and grammar masks ---------------------------------------------
 struct LogitsParams {
   const void *logits;

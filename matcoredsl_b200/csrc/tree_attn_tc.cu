@@ -1,0 +1,1012 @@
+// Attention of a tree of drafted tokens over a paged key/value cache, on
+// tcgen05 tensor cores: bf16 or f16, head size 64 or 128, 16-byte aligned rows.
+// (The mathematics and the masks: tree_attn.cu.)
+//
+// A unit is one request, one key head and up to ROWS of the request's rows
+// (row = new token x query heads of the group); its keys are cut into tiles of
+// 128. Every CTA (one per SM) takes an equal share of all units' tiles, in
+// order, so a long context is split over many CTAs and many short ones are
+// packed into one. The share is found on the device from the lengths: nothing
+// is read by the host. A unit that lies in one CTA is finished there; the parts
+// of a unit that spans CTAs go to scratch (at most two per CTA) and a second
+// launch joins them in their order.
+//
+// Two forms of a CTA, both with two softmax warpgroups g = 0, 1 (one thread a
+// row), each with its own scores S_g and output O_g in TMEM and weights P_g in
+// shared memory:
+//   kPair = false  128 rows; warpgroup g takes every second key tile, so that
+//                  the softmax of one tile overlaps the products of the next.
+//                  For few rows the time is the cache's read.
+//   kPair = true   256 rows, 128 for each warpgroup; each key tile is loaded
+//                  once for both. For wide trees and long runs of new tokens.
+// Warps 0-3 load (cp.async: pages may have any size and end inside a tile),
+// 4-7 and 8-11 are the warpgroups, warp 12 issues the products, warp 13 finds
+// the segments (a CTA's part of a unit) and hands them over a small ring.
+//
+// Keys that a row does not see get the score -inf. Their values must not reach
+// it either, and 0 x inf would: the loaders replace what is not finite in the
+// new tokens' values by 0, and the rows that do see such a value add it at
+// the end. Cache rows past the request's length are not read at all.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "internal.h"
+
+namespace mcb {
+namespace {
+
+constexpr int THREADS = 512;
+constexpr int BK = 128;                 // keys per tile
+constexpr int CHUNK_BYTES = 128 * 128;  // 128 rows x 64 16-bit columns, one swizzle span
+constexpr int LOADERS = 128;
+constexpr int SEGS = 4;         // ring of segments
+constexpr int VALID_RING = 16;  // key tiles whose validity words are kept
+constexpr int INFO_RING = 4;    // key tiles whose row numbers are kept
+constexpr int TMEM_COLS = 512;
+constexpr uint32_t S_COL = 0, O_COL = 256;
+
+template <int HD>
+constexpr int tile_bytes() {
+  return 128 * HD * 2;
+}
+template <int HD, bool kPair>
+constexpr int stages() {
+  return HD == 128 ? (kPair ? 3 : 4) : (kPair ? 6 : 8);
+}
+
+// A CTA's part of a unit.
+struct Segment {
+  int32_t kind;          // kWhole, kHead, kTail, or kEnd
+  int32_t b, head;       // request, key head
+  int32_t row0, nrows;   // rows of the request
+  int32_t tok0, n;       // first new token, number of new tokens
+  int32_t prefix, keys;  // position of the first new token; keys there are
+  int32_t tile0, ntiles;
+};
+enum : int32_t { kEnd = -1, kWhole = 0, kHead = 1, kTail = 2 };
+
+template <int HD, bool kPair>
+struct Smem {
+  static constexpr int ST = stages<HD, kPair>();
+  uint8_t q[kPair ? 2 : 1][tile_bytes<HD>()];
+  uint8_t kv[ST][tile_bytes<HD>()];
+  uint8_t p[2][128 * BK * 2];
+  int32_t info[INFO_RING][BK];  // cache row of each key of a tile, -1: none
+  uint32_t valid[VALID_RING][4];
+  Segment seg[SEGS];
+  uint64_t seg_full[SEGS], seg_empty[SEGS];
+  uint64_t q_full, q_empty;
+  uint64_t kv_full[ST], kv_empty[ST];
+  uint64_t s_full[2], s_free[2], p_full[2], p_free[2], o_full[2], o_empty[2];
+  uint64_t info_ready, join_full, join_read;
+  uint64_t drain;
+  int64_t start_b, start_w;
+  uint32_t tmem_slot;
+  int abort_flag, dirty;
+};
+constexpr size_t kMaxSmem = 232448;
+static_assert(sizeof(Smem<128, true>) <= kMaxSmem && sizeof(Smem<128, false>) <= kMaxSmem &&
+                  sizeof(Smem<64, true>) <= kMaxSmem && sizeof(Smem<64, false>) <= kMaxSmem,
+              "tree attention exceeds the shared memory per block");
+
+struct Params {
+  TreeAttn a;
+  float c;             // |scale| * log2(e)
+  uint32_t s_neg;      // negate A in the score product when scale < 0
+  uint32_t div_mul;    // row number / block = row * div_mul >> div_shift (row < 2^31)
+  int32_t div_shift;
+  float *partial;      // [2 * CTAs][ROWS][HD] outputs, then [2 * CTAs][ROWS][2] (max, sum)
+  TreeAttnPart *part;  // [CTAs]
+  uint32_t *status;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <bool kF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  return kF16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
+}
+__device__ __forceinline__ uint64_t kmajor_desc(uint32_t base, int kk) {
+  return make_sdesc_sw128(base + (kk >> 2) * CHUNK_BYTES + (kk & 3) * 32, 16, 1024);
+}
+__device__ __forceinline__ uint64_t mnmajor_desc(uint32_t base, int kk) {
+  return make_sdesc_sw128(base + kk * 2048, CHUNK_BYTES, 1024);
+}
+// 16 bytes to shared memory, zeros when `bytes` is 0.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// One request's lengths, clipped to the tensors.
+struct Request {
+  int32_t tok0, n, rows, prefix, keys;  // rows: of the tokens inside [0, T)
+};
+__device__ __forceinline__ Request load_request(const TreeAttn &a, int64_t b) {
+  Request r;
+  const int64_t c0 = a.cu[b], c1 = a.cu[b + 1], kv = max(0, a.kv_lens[b]);
+  const int64_t n = c0 >= 0 && c1 > c0 ? c1 - c0 : 0;
+  const int64_t in = max(static_cast<int64_t>(0), min(n, a.tokens - c0));
+  r.tok0 = static_cast<int32_t>(c0);
+  r.n = static_cast<int32_t>(n);
+  r.rows = static_cast<int32_t>(in * (a.heads / a.kv_heads));
+  r.prefix = static_cast<int32_t>(kv - n);
+  r.keys = static_cast<int32_t>(min(kv, a.columns * a.block));
+  return r;
+}
+// Key tiles of row tile `rt`: without a mask the rows see no key past the
+// last one's own.
+template <int ROWS>
+__device__ __forceinline__ int32_t unit_tiles(const TreeAttn &a, const Request &r, int32_t rt) {
+  int64_t end = r.keys;
+  if (!a.mask) {
+    const int32_t last = min(r.rows, (rt + 1) * ROWS) - 1;
+    end = min(end, static_cast<int64_t>(r.prefix) + last / (a.heads / a.kv_heads) + 1);
+  }
+  return end <= BK ? 1 : static_cast<int32_t>((end + BK - 1) / BK);
+}
+template <int ROWS>
+__device__ __forceinline__ int64_t head_tiles(const TreeAttn &a, const Request &r) {
+  const int32_t rts = (r.rows + ROWS - 1) / ROWS;
+  if (a.mask) return static_cast<int64_t>(rts) * (rts ? unit_tiles<ROWS>(a, r, 0) : 0);
+  int64_t sum = 0;
+  for (int32_t rt = 0; rt < rts; ++rt) sum += unit_tiles<ROWS>(a, r, rt);
+  return sum;
+}
+
+// Bits of the 32 keys from position pos on that new token i (mask row `row`)
+// may see; bit k is key pos + k.
+__device__ __forceinline__ uint32_t visible_word(const TreeAttn &a, const uint32_t *row,
+                                                 int32_t pos, int32_t prefix, int32_t i) {
+  const int64_t j = static_cast<int64_t>(pos) - prefix;  // new token of bit 0
+  if (j <= -32) return 0xffffffffu;
+  if (!row) {
+    const int64_t n = static_cast<int64_t>(i) - j + 1;  // keys up to the token itself
+    return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1;
+  }
+  auto word = [&](int64_t w) -> uint32_t { return w >= 0 && w < a.mask_words ? row[w] : 0u; };
+  if (j < 0) return (word(0) << -j) | ((1u << -j) - 1);
+  const int32_t s = static_cast<int32_t>(j & 31);
+  const uint32_t lo = word(j >> 5);
+  return s ? (lo >> s) | (word((j >> 5) + 1) << (32 - s)) : lo;
+}
+
+template <int HD, bool kPair, bool kF16>
+__global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p) {
+  constexpr int ST = stages<HD, kPair>();
+  constexpr int ROWS = kPair ? 256 : 128;
+  constexpr int AHEAD = kPair ? 1 : 2;  // score tiles issued before the first value tile
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  Smem<HD, kPair> &sm = *reinterpret_cast<Smem<HD, kPair> *>(smem_raw);
+  int64_t *scan = reinterpret_cast<int64_t *>(sm.info);  // before the roles start
+  const TreeAttn &a = p.a;
+  volatile int *abort_flag = &sm.abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = a.heads / a.kv_heads;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < SEGS; ++s) {
+      mbar_init(&sm.seg_full[s], 1);
+      mbar_init(&sm.seg_empty[s], LOADERS + 1 + 256);
+    }
+    mbar_init(&sm.q_full, LOADERS);
+    mbar_init(&sm.q_empty, 1);
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&sm.kv_full[s], LOADERS);
+      mbar_init(&sm.kv_empty[s], 1);
+    }
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(&sm.s_full[g], 1);
+      mbar_init(&sm.s_free[g], 128);
+      mbar_init(&sm.p_full[g], 128);
+      mbar_init(&sm.p_free[g], 1);
+      mbar_init(&sm.o_full[g], 1);
+      mbar_init(&sm.o_empty[g], 128);
+    }
+    mbar_init(&sm.info_ready, LOADERS);
+    mbar_init(&sm.join_full, 128);
+    mbar_init(&sm.join_read, 128);
+    mbar_init(&sm.drain, 1);
+    // The tiles' swizzle needs a 1024-byte aligned base.
+    sm.abort_flag = (smem_u32(smem_raw) & 1023u) != 0;
+    if (sm.abort_flag && p.status) atomicOr(p.status, kErrBadLaunch);
+    sm.dirty = 0;
+    fence_mbar_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(&sm.tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+
+  // ---- all tiles of all units, and this CTA's share [w0, w1) ----
+  const int64_t per_thread = (a.requests + THREADS - 1) / THREADS;
+  const int64_t b_first = threadIdx.x * per_thread;
+  const int64_t b_last = min(a.requests, b_first + per_thread);
+  int64_t mine = 0;
+  for (int64_t b = b_first; b < b_last; ++b)
+    mine += head_tiles<ROWS>(a, load_request(a, b)) * a.kv_heads;
+  int64_t incl = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int64_t o = __shfl_up_sync(0xffffffffu, incl, off);
+    if (lane >= off) incl += o;
+  }
+  if (lane == 31) scan[warp] = incl;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_slot;
+  int64_t total = 0, before = incl - mine;
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += scan[w];
+    total += scan[w];
+  }
+  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total);
+  const bool works = blockIdx.x < ctas && !sm.abort_flag;
+  const int64_t w0 = works ? blockIdx.x * total / ctas : 0;
+  const int64_t w1 = works ? (blockIdx.x + 1) * total / ctas : 0;
+  // The thread whose requests hold tile w0 leaves where they begin.
+  if (works && before <= w0 && w0 < before + mine) {
+    sm.start_b = b_first;
+    sm.start_w = before;
+  }
+  __syncthreads();
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    // ---------------- loaders ----------------
+    constexpr int PIECES = HD / 8;              // 16-byte pieces of a row
+    constexpr int STEP = LOADERS / PIECES;      // rows per pass
+    constexpr int PASSES = 128 / STEP;
+    const int l = threadIdx.x, piece = l % PIECES, r0 = l / PIECES;
+    // Offset of this thread's piece of row r0 in a tile; rows STEP apart have the
+    // same swizzle.
+    const uint32_t dst0 = (piece >> 3) * CHUNK_BYTES + r0 * 128 +
+                          (((piece & 7) ^ (r0 & 7)) << 4);
+    uint32_t kvc = 0, tiles = 0, sc = 0, described = 0;
+    uint32_t pend0 = 0, pend1 = 0;
+    int pending = 0;
+    bool ok = true;
+    // An item: 0 a query tile, 1 a key or value tile without further work, 2 a
+    // value tile whose rows from `first` on are new tokens'; its stage.
+    auto finish = [&](uint32_t item) {
+      const uint32_t type = item & 3, stage = (item >> 2) & 15, first = item >> 8;
+      if (type == 2) {
+        for (int it = 0; it < PASSES; ++it) {
+          if (r0 + it * STEP < static_cast<int>(first)) continue;
+          uint4 *at = reinterpret_cast<uint4 *>(sm.kv[stage] + dst0 + it * STEP * 128);
+          uint4 w = *at;
+          uint32_t *x = reinterpret_cast<uint32_t *>(&w);
+          bool bad = false;
+          constexpr uint32_t E = kF16 ? 0x7c00u : 0x7f80u;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if ((x[i] & E) == E) {
+              x[i] &= 0xffff0000u;
+              bad = true;
+            }
+            if ((x[i] & (E << 16)) == (E << 16)) {
+              x[i] &= 0xffffu;
+              bad = true;
+            }
+          }
+          if (bad) {
+            *at = w;
+            *static_cast<volatile int *>(&sm.dirty) = 1;
+          }
+        }
+      }
+      fence_async_smem();
+      mbar_arrive(type == 0 ? &sm.q_full : &sm.kv_full[stage]);
+    };
+    auto flush = [&] {
+      if (pending == 0) return;
+      cp_async_wait<0>();
+      finish(pend0);
+      if (pending == 2) finish(pend1);
+      pending = 0;
+    };
+    auto push = [&](uint32_t item) {
+      cp_async_commit();
+      if (pending == 2) {
+        cp_async_wait<2>();
+        finish(pend0);
+        pend0 = pend1;
+        pend1 = item;
+      } else if (pending == 1) {
+        pend1 = item;
+        pending = 2;
+      } else {
+        pend0 = item;
+        pending = 1;
+      }
+    };
+    // Blocks on a barrier only with nothing held back: what is waited for may
+    // need the items still in flight.
+    auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
+      bool got = mbar_try_wait(smem_u32(bar), parity);
+      if (!got) {
+        flush();
+        got = mbar_wait(bar, parity, abort_flag, p.status, kErrTimeoutEmpty);
+      }
+      return __all_sync(0xffffffffu, got) != 0;  // a warp goes on or ends as one
+    };
+    for (; ok; ++sc) {
+      const int ss = sc % SEGS;
+      if (!(ok = wait(&sm.seg_full[ss], (sc / SEGS) & 1))) break;
+      const Segment sg = sm.seg[ss];
+      mbar_arrive(&sm.seg_empty[ss]);
+      if (sg.kind == kEnd) break;
+      // ---- queries ----
+      if (!(ok = wait(&sm.q_empty, (sc & 1) ^ 1))) break;
+      {
+        const char *q = static_cast<const char *>(a.q) + piece * 16;
+        for (int it = 0; it < PASSES * (kPair ? 2 : 1); ++it) {
+          const int r = r0 + it * STEP;
+          const int row = sg.row0 + r, tok = row / group;
+          const bool live = r < sg.nrows;
+          const char *src = live ? q + ((static_cast<int64_t>(sg.tok0) + tok) * a.q_s[0] +
+                                        (static_cast<int64_t>(sg.head) * group + row - tok * group) *
+                                            a.q_s[1]) * 2
+                                 : q;
+          cp_async16(smem_u32(sm.q[r >> 7]) + dst0 + (it % PASSES) * STEP * 128, src, live ? 16 : 0);
+        }
+        push(0);
+      }
+      // ---- keys and values ----
+      const int32_t *table = a.table + sg.b * a.table_stride;
+      const int key0 = sg.tile0 * BK;
+      auto entry = [&](int j) -> int32_t {  // block of this thread's key of tile j
+        const int key = key0 + j * BK + l;
+        if (j >= sg.ntiles || key >= sg.keys) return -1;
+        return table[static_cast<uint32_t>(
+            (static_cast<uint64_t>(key) * p.div_mul) >> p.div_shift)];
+      };
+      int32_t next = entry(0);
+      auto describe = [&](int j) -> bool {
+        const int key = key0 + j * BK + l;
+        const int32_t blk = next;
+        next = entry(j + 1);
+        const uint32_t col = static_cast<uint32_t>(
+            (static_cast<uint64_t>(key) * p.div_mul) >> p.div_shift);
+        const bool good = key < sg.keys && blk >= 0 && blk < a.blocks;
+        sm.info[j % INFO_RING][l] = good ? blk * a.block + (key - static_cast<int>(col) * a.block) : -1;
+        const uint32_t bits = __ballot_sync(0xffffffffu, good);
+        if (lane == 0) sm.valid[(tiles + j) % VALID_RING][warp] = bits;
+        mbar_arrive(&sm.info_ready);
+        // Nothing is held up by items in flight here: every loader gets here
+        // without waiting for anything that this one has not waited for.
+        return __all_sync(0xffffffffu, mbar_wait(&sm.info_ready, described++ & 1, abort_flag,
+                                                 p.status, kErrTimeoutEmpty)) != 0;
+      };
+      auto load = [&](int j, bool value) -> bool {
+        const int s = kvc % ST;
+        if (!wait(&sm.kv_empty[s], ((kvc / ST) & 1) ^ 1)) return false;
+        ++kvc;
+        const int64_t *st = value ? a.v_s : a.k_s;
+        const char *base = static_cast<const char *>(value ? a.v : a.k) + sg.head * st[2] * 2 +
+                           piece * 16;
+        const uint32_t dst = smem_u32(sm.kv[s]) + dst0;
+#pragma unroll
+        for (int it = 0; it < PASSES; ++it) {
+          const int32_t row = sm.info[j % INFO_RING][r0 + it * STEP];
+          const char *src = base;
+          if (row >= 0) {
+            const uint32_t blk = static_cast<uint32_t>(
+                (static_cast<uint64_t>(row) * p.div_mul) >> p.div_shift);
+            src += (blk * st[0] + (row - static_cast<int32_t>(blk) * a.block) * st[1]) * 2;
+          }
+          cp_async16(dst + it * STEP * 128, src, row >= 0 ? 16 : 0);
+        }
+        const int first = min(max(sg.prefix - (key0 + j * BK), 0), BK);
+        push((value && first < BK ? 2u : 1u) | (static_cast<uint32_t>(s) << 2) |
+             (static_cast<uint32_t>(first) << 8));
+        return true;
+      };
+      for (int j = 0; j < AHEAD && j < sg.ntiles && ok; ++j) {
+        ok = describe(j) && load(j, false);
+      }
+      for (int j = 0; j < sg.ntiles && ok; ++j) {
+        if (j + AHEAD < sg.ntiles) {
+          ok = describe(j + AHEAD) && load(j + AHEAD, false);
+        }
+        ok = ok && load(j, true);
+      }
+      tiles += sg.ntiles;
+      if (!ok) break;
+    }
+    flush();
+  } else if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 12 && lane == 0) {
+      // ---------------- MMA issuer ----------------
+      constexpr uint32_t F = kF16 ? 0 : 1;
+      const uint32_t idesc_s = make_idesc(F, F, 0, 0, 128, BK) | p.s_neg;
+      const uint32_t idesc_o = make_idesc(F, F, 0, 1, 128, HD);
+      uint32_t kvc = 0, sc = 0, s_cnt[2] = {0, 0}, p_cnt[2] = {0, 0}, o_cnt[2] = {0, 0};
+      bool ok = true;
+      for (; ok; ++sc) {
+        const int ss = sc % SEGS;
+        if (!mbar_wait(&sm.seg_full[ss], (sc / SEGS) & 1, abort_flag, p.status, kErrTimeoutFull))
+          break;
+        const Segment sg = sm.seg[ss];
+        mbar_arrive(&sm.seg_empty[ss]);
+        if (sg.kind == kEnd) break;
+        const int n = sg.ntiles;
+        const int groups = sg.nrows > 128 ? 2 : 1;  // kPair: warpgroups with rows
+        if (!mbar_wait(&sm.q_full, sc & 1, abort_flag, p.status, kErrTimeoutFull)) break;
+        tc_fence_after();
+        // Scores of tile j: for both row halves, or for the tile's warpgroup.
+        auto scores = [&](int j) -> bool {
+          const int s = kvc % ST;
+          if (!mbar_wait(&sm.kv_full[s], (kvc / ST) & 1, abort_flag, p.status, kErrTimeoutFull))
+            return false;
+          ++kvc;
+          const uint32_t k_addr = smem_u32(sm.kv[s]);
+          const int g0 = kPair ? 0 : (j & 1), g1 = kPair ? groups : g0 + 1;
+          for (int g = g0; g < g1; ++g) {
+            if (!mbar_wait(&sm.s_free[g], (s_cnt[g] & 1) ^ 1, abort_flag, p.status,
+                           kErrTimeoutAccum))
+              return false;
+            ++s_cnt[g];
+            tc_fence_after();
+            const uint32_t q_addr = smem_u32(sm.q[kPair ? g : 0]);
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk)
+              mma_f16_ss(tmem + S_COL + g * BK, kmajor_desc(q_addr, kk), kmajor_desc(k_addr, kk),
+                         idesc_s, kk ? 1u : 0u);
+            mma_commit(&sm.s_full[g]);
+          }
+          mma_commit(&sm.kv_empty[s]);
+          return true;
+        };
+        auto values = [&](int j) -> bool {
+          const int s = kvc % ST;
+          if (!mbar_wait(&sm.kv_full[s], (kvc / ST) & 1, abort_flag, p.status, kErrTimeoutFull))
+            return false;
+          ++kvc;
+          const uint32_t v_addr = smem_u32(sm.kv[s]);
+          const int g0 = kPair ? 0 : (j & 1), g1 = kPair ? groups : g0 + 1;
+          for (int g = g0; g < g1; ++g) {
+            const bool first = kPair ? j == 0 : j < 2;
+            const bool last = kPair ? j + 1 == n : j + 2 >= n;
+            if (first) {
+              if (!mbar_wait(&sm.o_empty[g], (o_cnt[g] & 1) ^ 1, abort_flag, p.status,
+                             kErrTimeoutAccum))
+                return false;
+              ++o_cnt[g];
+            }
+            if (!mbar_wait(&sm.p_full[g], p_cnt[g] & 1, abort_flag, p.status, kErrTimeoutAccum))
+              return false;
+            ++p_cnt[g];
+            tc_fence_after();
+            const uint32_t p_addr = smem_u32(sm.p[g]);
+#pragma unroll
+            for (int kk = 0; kk < BK / 16; ++kk)
+              mma_f16_ss(tmem + O_COL + g * HD, kmajor_desc(p_addr, kk), mnmajor_desc(v_addr, kk),
+                         idesc_o, (!first || kk) ? 1u : 0u);
+            mma_commit(&sm.p_free[g]);
+            if (last) mma_commit(&sm.o_full[g]);
+          }
+          mma_commit(&sm.kv_empty[s]);
+          return true;
+        };
+        for (int j = 0; j < AHEAD && j < n && ok; ++j) ok = scores(j);
+        if (ok && n <= AHEAD) mma_commit(&sm.q_empty);
+        for (int j = 0; j < n && ok; ++j) {
+          if (j + AHEAD < n) {
+            ok = scores(j + AHEAD);
+            if (ok && j + AHEAD + 1 == n) mma_commit(&sm.q_empty);
+          }
+          ok = ok && values(j);
+        }
+      }
+      mma_commit(&sm.drain);
+      if (!mbar_wait(&sm.drain, 0, nullptr, p.status, kErrTimeoutDrain)) *abort_flag = 1;
+    } else if (warp == 13 && lane == 0) {
+      // ---------------- scheduler ----------------
+      uint32_t sc = 0;
+      bool ok = true;
+      TreeAttnPart part{};
+      auto put = [&](const Segment &sg) -> bool {
+        const int ss = sc % SEGS;
+        if (!mbar_wait(&sm.seg_empty[ss], ((sc / SEGS) & 1) ^ 1, abort_flag, p.status,
+                       kErrTimeoutEmpty))
+          return false;
+        sm.seg[ss] = sg;
+        mbar_arrive(&sm.seg_full[ss]);
+        ++sc;
+        return true;
+      };
+      if (w0 < w1) {
+        int64_t w = w0, b = sm.start_b, at = sm.start_w;  // `at`: first tile of request b
+        Request r = load_request(a, b);
+        int64_t per = head_tiles<ROWS>(a, r);
+        while (at + per * a.kv_heads <= w) {
+          at += per * a.kv_heads;
+          r = load_request(a, ++b);
+          per = head_tiles<ROWS>(a, r);
+        }
+        int32_t head = static_cast<int32_t>((w - at) / per), rt = 0;
+        int64_t rest = w - at - head * per;
+        int32_t n = unit_tiles<ROWS>(a, r, 0);
+        while (rest >= n) {
+          rest -= n;
+          n = unit_tiles<ROWS>(a, r, ++rt);
+        }
+        int32_t tile0 = static_cast<int32_t>(rest);
+        while (ok) {
+          const int32_t take = static_cast<int32_t>(min(static_cast<int64_t>(n - tile0), w1 - w));
+          const bool ends = tile0 + take == n;
+          Segment sg;
+          sg.kind = tile0 > 0 ? kHead : ends ? kWhole : kTail;
+          sg.b = static_cast<int32_t>(b);
+          sg.head = head;
+          sg.row0 = rt * ROWS;
+          sg.nrows = min(r.rows - sg.row0, ROWS);
+          sg.tok0 = r.tok0;
+          sg.n = r.n;
+          sg.prefix = r.prefix;
+          sg.keys = r.keys;
+          sg.tile0 = tile0;
+          sg.ntiles = take;
+          if (sg.kind == kTail) {
+            // Last CTA with a part of this unit.
+            const int64_t last = w - tile0 + n - 1;
+            part.parts = static_cast<int32_t>(((last + 1) * ctas - 1) / total - blockIdx.x) + 1;
+            part.tok0 = r.tok0;
+            part.head = head;
+            part.row0 = sg.row0;
+            part.nrows = sg.nrows;
+          }
+          ok = put(sg);
+          w += take;
+          if (w >= w1 || !ok) break;
+          tile0 = 0;
+          if ((rt + 1) * ROWS < r.rows) {
+            n = unit_tiles<ROWS>(a, r, ++rt);
+            continue;
+          }
+          rt = 0;
+          if (++head == a.kv_heads) {
+            head = 0;
+            do r = load_request(a, ++b);
+            while (r.rows == 0);
+          }
+          n = unit_tiles<ROWS>(a, r, 0);
+        }
+      }
+      p.part[blockIdx.x] = part;
+      Segment end{};
+      end.kind = kEnd;
+      if (ok) put(end);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    // ---------------- softmax and output ----------------
+    const int g = (warp - 4) >> 2, sub = warp & 3;
+    const int row = sub * 32 + lane;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(sub * 32) << 16);
+    const uint32_t s_col = S_COL + g * BK, o_col = O_COL + g * HD;
+    uint8_t *p_row = sm.p[g] + row * 128;
+    const int rsw = row & 7;
+    uint32_t sc = 0, s_cnt = 0, p_cnt = 0, o_cnt[2] = {0, 0}, tiles = 0, joins = 0;
+    bool ok = true;
+    for (; ok; ++sc) {
+      const int ss = sc % SEGS;
+      if (!(ok = mbar_wait_warp(&sm.seg_full[ss], (sc / SEGS) & 1, abort_flag, p.status,
+                                kErrTimeoutAccum)))
+        break;
+      const Segment sg = sm.seg[ss];
+      mbar_arrive(&sm.seg_empty[ss]);
+      if (sg.kind == kEnd) break;
+      const int n = sg.ntiles;
+      const int base = kPair ? g * 128 : 0;       // first unit row of this warpgroup
+      const int step = kPair ? 1 : 2, j0 = kPair ? 0 : g;
+      const bool joined = !kPair && n > 1;        // both warpgroups hold a part of each row
+      const bool busy = kPair ? base < sg.nrows : g < n;
+      const bool live = base + sub * 32 < sg.nrows;  // this warp has rows
+      const int urow = min(sg.row0 + base + row, sg.row0 + sg.nrows - 1);
+      const int i = urow / group;                    // new token of this row
+      const uint32_t *mask_row =
+          a.mask ? a.mask + (static_cast<int64_t>(sg.tok0) + i) * a.mask_stride : nullptr;
+      float m_ref = -INFINITY, l = 0.0f;
+      for (int j = j0; j < n && busy; j += step) {
+        if (!(ok = mbar_wait_warp(&sm.s_full[g], s_cnt & 1, abort_flag, p.status,
+                                  kErrTimeoutAccum)))
+          break;
+        ++s_cnt;
+        tc_fence_after();
+        if (!live) {  // no rows: hand the tile on
+          mbar_arrive(&sm.s_free[g]);
+          if (!(ok = mbar_wait_warp(&sm.p_free[g], (p_cnt & 1) ^ 1, abort_flag, p.status,
+                                    kErrTimeoutAccum)))
+            break;
+          mbar_arrive(&sm.p_full[g]);
+          ++p_cnt;
+          continue;
+        }
+        uint32_t s[128];
+        {
+          uint32_t (&s0)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[0]);
+          uint32_t (&s1)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[32]);
+          uint32_t (&s2)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[64]);
+          uint32_t (&s3)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[96]);
+          const uint32_t at = lane_base + s_col;
+          tmem_ld_32x32b_x32(at, s0);
+          tmem_ld_32x32b_x32(at + 32, s1);
+          tmem_ld_32x32b_x32(at + 64, s2);
+          tmem_ld_32x32b_x32(at + 96, s3);
+          tmem_ld_wait();
+          reg_fence(s0);
+          reg_fence(s1);
+          reg_fence(s2);
+          reg_fence(s3);
+        }
+        tc_fence_before();
+        mbar_arrive(&sm.s_free[g]);
+        const int pos0 = (sg.tile0 + j) * BK;
+        const uint4 good = *reinterpret_cast<const uint4 *>(sm.valid[(tiles + j) % VALID_RING]);
+        if (pos0 + BK > sg.prefix || (good.x & good.y & good.z & good.w) != 0xffffffffu) {
+          const uint32_t gw[4] = {good.x, good.y, good.z, good.w};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t see = gw[w] & visible_word(a, mask_row, pos0 + 32 * w, sg.prefix, i);
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (!((see >> k) & 1u)) s[32 * w + k] = 0xff800000u;
+          }
+        }
+        float m4[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m4[k] = __uint_as_float(s[k]);
+#pragma unroll
+        for (int k = 4; k < 128; k += 8)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            m4[q] = fmax3(m4[q], __uint_as_float(s[(k + 2 * q) & 127]),
+                          __uint_as_float(s[(k + 2 * q + 1) & 127]));
+        const float mx = fmax3(m4[0], m4[1], fmaxf(m4[2], m4[3]));
+        // The reference maximum moves only when a weight would pass 2^8. While
+        // it is -inf, O and l are zero.
+        bool need = false;
+        if (m_ref == -INFINITY)
+          m_ref = mx > -INFINITY ? mx : -INFINITY;
+        else
+          need = (mx - m_ref) * p.c > 8.0f;
+        if (__any_sync(0xffffffffu, need)) {
+          if (!(ok = mbar_wait_warp(&sm.p_free[g], (p_cnt - 1) & 1, abort_flag, p.status,
+                                    kErrTimeoutAccum)))
+            break;
+          tc_fence_after();
+          const float f = need ? ex2((m_ref - mx) * p.c) : 1.0f;
+#pragma unroll 1
+          for (int c0 = 0; c0 < HD; c0 += 16) {
+            uint32_t o[16];
+            tmem_ld16_sync(lane_base + o_col + c0, o);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+            tmem_st_32x32b_x16(lane_base + o_col + c0, o);
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          if (need) {
+            l *= f;
+            m_ref = mx;
+          }
+        }
+        const float mc = m_ref == -INFINITY ? 0.0f : m_ref * p.c;
+        const uint64_t c2 = f2_pack(p.c, p.c), nmc2 = f2_pack(-mc, -mc);
+        uint32_t pk[64];
+        uint64_t ps[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < 64; ++k) {
+          float x0, x1;
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), c2,
+                           nmc2),
+                    x0, x1);
+          const float e0 = ex2(x0), e1 = ex2(x1);
+          ps[k & 3] = f2_add(ps[k & 3], f2_pack(e0, e1));
+          pk[k] = pack2<kF16>(e0, e1);
+        }
+        {
+          float a0, a1;
+          f2_unpack(f2_add(f2_add(ps[0], ps[1]), f2_add(ps[2], ps[3])), a0, a1);
+          l += a0 + a1;
+        }
+        if (!(ok = mbar_wait_warp(&sm.p_free[g], (p_cnt & 1) ^ 1, abort_flag, p.status,
+                                  kErrTimeoutAccum)))
+          break;
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+          const int chunk = u >> 3, q = u & 7;
+          *reinterpret_cast<uint4 *>(p_row + chunk * CHUNK_BYTES + ((q ^ rsw) << 4)) =
+              make_uint4(pk[u * 4], pk[u * 4 + 1], pk[u * 4 + 2], pk[u * 4 + 3]);
+        }
+        fence_async_smem();
+        mbar_arrive(&sm.p_full[g]);
+        ++p_cnt;
+      }
+      if (!ok) break;
+      tiles += n;
+      // ---- output ----
+      if (!busy) continue;
+      float mc = m_ref == -INFINITY ? -INFINITY : m_ref * p.c;
+      float w_own = 1.0f, w_other = 0.0f;
+      for (int h = 0; h < 2; ++h) {
+        if (h != g && !(joined && g == 0)) continue;
+        if (!(ok = mbar_wait_warp(&sm.o_full[h], o_cnt[h] & 1, abort_flag, p.status,
+                                  kErrTimeoutAccum)))
+          break;
+        ++o_cnt[h];
+      }
+      if (!ok) break;
+      tc_fence_after();
+      if (joined) {
+        // Warpgroup 1 leaves its maximum and sum in its weights' buffer (free
+        // after its last product) and is done; warpgroup 0 reads both outputs,
+        // whose rows lie in the same TMEM lanes.
+        float2 *shared = reinterpret_cast<float2 *>(sm.p[1]);
+        if (g == 1) {
+          shared[row] = make_float2(mc, l);
+          mbar_arrive(&sm.join_full);
+          // The buffer may be written again once it has been read.
+          if (!(ok = mbar_wait_warp(&sm.join_read, joins++ & 1, abort_flag, p.status,
+                                    kErrTimeoutAccum)))
+            break;
+          continue;
+        }
+        if (!(ok = mbar_wait_warp(&sm.join_full, joins++ & 1, abort_flag, p.status,
+                                  kErrTimeoutAccum)))
+          break;
+        const float2 other = shared[row];
+        mbar_arrive(&sm.join_read);
+        const float top = fmaxf(mc, other.x), ref = top == -INFINITY ? 0.0f : top;
+        w_own = ex2(mc - ref);
+        w_other = ex2(other.x - ref);
+        l = l * w_own + other.y * w_other;
+        mc = top;
+      }
+      if (live) {
+        const bool mine_live = base + row < sg.nrows;
+        const bool dirty = *static_cast<volatile int *>(&sm.dirty) != 0;
+        const int64_t tok = static_cast<int64_t>(sg.tok0) + i;
+        const int head = sg.head * group + urow - i * group;
+        const bool whole = sg.kind == kWhole;
+        const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+        const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (sg.kind == kTail);
+        char *orow = static_cast<char *>(a.o) + (tok * a.o_s[0] + head * a.o_s[1]) * 2;
+        float *prow = p.partial + (slot * ROWS + base + row) * HD;
+#pragma unroll 1
+        for (int c0 = 0; c0 < HD; c0 += 32) {
+          uint32_t o[32];
+          tmem_ld32_sync(lane_base + o_col + c0, o);
+          float x[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k) x[k] = __uint_as_float(o[k]);
+          if (joined) {
+            tmem_ld32_sync(lane_base + O_COL + HD + c0, o);
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              x[k] = x[k] * w_own + __uint_as_float(o[k]) * w_other;
+          }
+          if (dirty) {
+            // Values of new tokens that are not finite, where the row sees them.
+            const int k0 = max(sg.tile0 * BK, sg.prefix);
+            const int k1 = min((sg.tile0 + n) * BK, sg.keys);
+            for (int pos = max(k0, 0); pos < k1; ++pos) {
+              if (!(visible_word(a, mask_row, pos, sg.prefix, i) & 1u)) continue;
+              const int col = pos / a.block;
+              const int32_t blk = a.table[sg.b * a.table_stride + col];
+              if (blk < 0 || blk >= a.blocks) continue;
+              const int64_t at = blk * a.v_s[0] +
+                                 static_cast<int64_t>(pos - col * a.block) * a.v_s[1] +
+                                 sg.head * a.v_s[2] + c0;
+#pragma unroll
+              for (int k = 0; k < 32; ++k) {
+                const float v =
+                    kF16 ? __half2float(static_cast<const __half *>(a.v)[at + k])
+                         : __bfloat162float(static_cast<const __nv_bfloat16 *>(a.v)[at + k]);
+                if (!(fabsf(v) < INFINITY)) x[k] += v;
+              }
+            }
+          }
+          if (mine_live) {
+            if (whole) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<uint4 *>(orow + (c0 + 8 * q) * 2) = make_uint4(
+                    pack2<kF16>(x[8 * q] * inv, x[8 * q + 1] * inv),
+                    pack2<kF16>(x[8 * q + 2] * inv, x[8 * q + 3] * inv),
+                    pack2<kF16>(x[8 * q + 4] * inv, x[8 * q + 5] * inv),
+                    pack2<kF16>(x[8 * q + 6] * inv, x[8 * q + 7] * inv));
+            } else {
+#pragma unroll
+              for (int q = 0; q < 8; ++q)
+                *reinterpret_cast<float4 *>(prow + c0 + 4 * q) =
+                    make_float4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
+            }
+          }
+        }
+        if (mine_live) {
+          if (whole) {
+            if (a.lse)
+              a.lse[tok * a.lse_s + head] =
+                  l == 0.0f ? -INFINITY
+                            : ((mc == -INFINITY ? 0.0f : mc) + log2f(l)) * 0.69314718055994531f;
+          } else {
+            float2 *ml = reinterpret_cast<float2 *>(
+                p.partial + static_cast<int64_t>(gridDim.x) * 2 * ROWS * HD);
+            ml[slot * ROWS + base + row] = make_float2(mc, l);
+          }
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(&sm.o_empty[g]);
+      if (joined) mbar_arrive(&sm.o_empty[1]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// Joins the parts of the units that span CTAs, in their order, one warp a row;
+// the last column of CTAs clears the tokens of no request.
+template <int HD, int ROWS, bool kF16>
+__global__ void __launch_bounds__(256) tree_attn_tc_join_kernel(const Params p, int ctas) {
+  const TreeAttn &a = p.a;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int group = a.heads / a.kv_heads;
+  if (blockIdx.x == ctas) {
+    const int64_t c0 = min(max(static_cast<int64_t>(a.cu[0]), static_cast<int64_t>(0)), a.tokens);
+    const int64_t c1 = max(c0, min(static_cast<int64_t>(a.cu[a.requests]), a.tokens));
+    const int64_t none = c0 + a.tokens - c1;  // tokens before the first and after the last request
+    for (int64_t w = blockIdx.y * 8 + warp; w < none * a.heads; w += 8 * gridDim.y) {
+      const int64_t at = w / a.heads, h = w - at * a.heads, t = at < c0 ? at : at - c0 + c1;
+      uint32_t *o = reinterpret_cast<uint32_t *>(static_cast<char *>(a.o) +
+                                                 (t * a.o_s[0] + h * a.o_s[1]) * 2);
+      for (int d = lane; d < HD / 2; d += 32) o[d] = 0;
+      if (lane == 0 && a.lse) a.lse[t * a.lse_s + h] = -INFINITY;
+    }
+    return;
+  }
+  const TreeAttnPart part = p.part[blockIdx.x];
+  if (part.parts == 0) return;
+  const float2 *ml = reinterpret_cast<const float2 *>(p.partial +
+                                                      static_cast<int64_t>(ctas) * 2 * ROWS * HD);
+  // Part k: the tail slot of this CTA, then the head slots of the next ones.
+  auto slot = [&](int k) -> int64_t {
+    return (static_cast<int64_t>(blockIdx.x) + k) * 2 + (k == 0);
+  };
+  constexpr int V = HD / 32;
+  for (int r = blockIdx.y * 8 + warp; r < part.nrows; r += 8 * gridDim.y) {
+    float top = -INFINITY;
+    for (int k = lane; k < part.parts; k += 32) top = fmaxf(top, ml[slot(k) * ROWS + r].x);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float l = 0.0f, x[V] = {};
+#pragma unroll 4
+    for (int k = 0; k < part.parts; ++k) {
+      const float2 z = ml[slot(k) * ROWS + r];
+      const float w = ex2(z.x - ref);
+      l += z.y * w;
+      const float *in = p.partial + (slot(k) * ROWS + r) * HD + lane * V;
+      float y[V];
+      if (V == 4) {
+        const float4 f = *reinterpret_cast<const float4 *>(in);
+        y[0] = f.x, y[1] = f.y, y[V - 2] = f.z, y[V - 1] = f.w;
+      } else {
+        const float2 f = *reinterpret_cast<const float2 *>(in);
+        y[0] = f.x, y[1] = f.y;
+      }
+#pragma unroll
+      for (int d = 0; d < V; ++d) x[d] = fmaf(y[d], w, x[d]);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int row = part.row0 + r, i = row / group;
+    const int64_t tok = static_cast<int64_t>(part.tok0) + i;
+    const int head = part.head * group + row - i * group;
+    uint32_t *o = reinterpret_cast<uint32_t *>(static_cast<char *>(a.o) +
+                                               (tok * a.o_s[0] + head * a.o_s[1]) * 2);
+#pragma unroll
+    for (int d = 0; d < V / 2; ++d)
+      o[lane * (V / 2) + d] = pack2<kF16>(x[2 * d] * inv, x[2 * d + 1] * inv);
+    if (lane == 0 && a.lse)
+      a.lse[tok * a.lse_s + head] =
+          l == 0.0f ? -INFINITY : (ref + log2f(l)) * 0.69314718055994531f;
+  }
+}
+
+bool pair_of(const TreeAttn &a) {
+  // Two row halves per CTA when a request has more than 128 rows on average.
+  return a.tokens * (a.heads / a.kv_heads) > 128 * a.requests;
+}
+
+template <int HD, bool kPair, bool kF16>
+cudaError_t run(const Params &p, int ctas, cudaStream_t stream) {
+  constexpr int ROWS = kPair ? 256 : 128;
+  auto kernel = tree_attn_tc_kernel<HD, kPair, kF16>;
+  constexpr int smem = static_cast<int>(sizeof(Smem<HD, kPair>));
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  kernel<<<ctas, THREADS, smem, stream>>>(p);
+  tree_attn_tc_join_kernel<HD, ROWS, kF16><<<dim3(ctas + 1, 8), 256, 0, stream>>>(p, ctas);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+bool tree_attn_tc_ok(const TreeAttn &a, int dtype) {
+  if (dtype != MCB_DTYPE_BF16 && dtype != MCB_DTYPE_F16) return false;
+  if (a.dim != 64 && a.dim != 128) return false;
+  if (a.scale == 0.0f) return false;  // a masked score times 0 would be NaN
+  const uintptr_t bases = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) |
+                          reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.o);
+  int64_t steps = a.q_s[0] | a.q_s[1] | a.o_s[0] | a.o_s[1];
+  for (int i = 0; i < 3; ++i) steps |= a.k_s[i] | a.v_s[i];
+  return bases % 16 == 0 && steps % 8 == 0 && a.tokens * a.heads <= 0x7fffffff &&
+         a.columns * a.block <= 0x7fffff00;
+}
+
+uint64_t tree_attn_tc_scratch(const TreeAttn &a, int sms) {
+  const uint64_t rows = pair_of(a) ? 256 : 128;
+  return static_cast<uint64_t>(sms) * (2 * rows * (a.dim + 2) * sizeof(float) + sizeof(TreeAttnPart));
+}
+
+cudaError_t launch_tree_attn_tc(const TreeAttn &a, int dtype, void *scratch, uint32_t *status,
+                                int sms, cudaStream_t stream, LaunchInfo *info) {
+  const bool pair = pair_of(a), f16 = dtype == MCB_DTYPE_F16;
+  Params p;
+  p.a = a;
+  p.c = fabsf(a.scale) * 1.4426950408889634f;
+  p.s_neg = a.scale < 0.0f ? kIdescNegateA : 0u;
+  // x / d for x < 2^31: x * ceil(2^(31+s) / d) >> (31+s) with 2^s >= d.
+  int s = 0;
+  while ((static_cast<int64_t>(1) << s) < a.block) ++s;
+  p.div_shift = 31 + s;
+  p.div_mul = static_cast<uint32_t>(
+      ((static_cast<uint64_t>(1) << (31 + s)) + a.block - 1) / static_cast<uint64_t>(a.block));
+  p.partial = static_cast<float *>(scratch);
+  p.part = reinterpret_cast<TreeAttnPart *>(
+      p.partial + static_cast<uint64_t>(sms) * 2 * (pair ? 256 : 128) * (a.dim + 2));
+  p.status = status;
+  cudaError_t e;
+  auto pick = [&](auto run_bf16, auto run_f16) {
+    return f16 ? run_f16(p, sms, stream) : run_bf16(p, sms, stream);
+  };
+  if (a.dim == 128)
+    e = pair ? pick(run<128, true, false>, run<128, true, true>)
+             : pick(run<128, false, false>, run<128, false, true>);
+  else
+    e = pair ? pick(run<64, true, false>, run<64, true, true>)
+             : pick(run<64, false, false>, run<64, false, true>);
+  info->launches = 2;
+  info->tile_m = pair ? 256 : 128;
+  info->tile_n = BK;
+  info->tile_k = a.dim;
+  info->stages = a.dim == 128 ? (pair ? stages<128, true>() : stages<128, false>())
+                              : (pair ? stages<64, true>() : stages<64, false>());
+  info->ctas = sms;
+  info->set_route("tcgen05_tree_attention");
+  return e;
+}
+
+}  // namespace mcb
