@@ -122,12 +122,15 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int by
                "r"(bytes)
                : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() {
-  asm volatile("cp.async.commit_group;" ::: "memory");
+// One arrival on `bar` once this thread's copies so far have landed. The
+// copies are generic-proxy writes: whoever waits on the barrier fences before a
+// tensor-core instruction reads them.
+__device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
 }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ void cp_async_wait_all() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // One request's lengths, clipped to the tensors.
@@ -276,72 +279,37 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
     const uint32_t dst0 = (piece >> 3) * CHUNK_BYTES + r0 * 128 +
                           (((piece & 7) ^ (r0 & 7)) << 4);
     uint32_t kvc = 0, tiles = 0, sc = 0, described = 0;
-    uint32_t pend0 = 0, pend1 = 0;
-    int pending = 0;
     bool ok = true;
-    // An item: 0 a query tile, 1 a key or value tile without further work, 2 a
-    // value tile whose rows from `first` on are new tokens'; its stage.
-    auto finish = [&](uint32_t item) {
-      const uint32_t type = item & 3, stage = (item >> 2) & 15, first = item >> 8;
-      if (type == 2) {
-        for (int it = 0; it < PASSES; ++it) {
-          if (r0 + it * STEP < static_cast<int>(first)) continue;
-          uint4 *at = reinterpret_cast<uint4 *>(sm.kv[stage] + dst0 + it * STEP * 128);
-          uint4 w = *at;
-          uint32_t *x = reinterpret_cast<uint32_t *>(&w);
-          bool bad = false;
-          constexpr uint32_t E = kF16 ? 0x7c00u : 0x7f80u;
+    auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status,
+                                               kErrTimeoutEmpty)) != 0;
+    };
+    // This thread's pieces of a value tile whose rows from `first` on are new
+    // tokens': what is not finite becomes 0.
+    auto clean = [&](uint8_t *tile, int first) {
+      for (int it = 0; it < PASSES; ++it) {
+        if (r0 + it * STEP < first) continue;
+        uint4 *at = reinterpret_cast<uint4 *>(tile + dst0 + it * STEP * 128);
+        uint4 w = *at;
+        uint32_t *x = reinterpret_cast<uint32_t *>(&w);
+        bool bad = false;
+        constexpr uint32_t E = kF16 ? 0x7c00u : 0x7f80u;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if ((x[i] & E) == E) {
-              x[i] &= 0xffff0000u;
-              bad = true;
-            }
-            if ((x[i] & (E << 16)) == (E << 16)) {
-              x[i] &= 0xffffu;
-              bad = true;
-            }
+        for (int i = 0; i < 4; ++i) {
+          if ((x[i] & E) == E) {
+            x[i] &= 0xffff0000u;
+            bad = true;
           }
-          if (bad) {
-            *at = w;
-            *static_cast<volatile int *>(&sm.dirty) = 1;
+          if ((x[i] & (E << 16)) == (E << 16)) {
+            x[i] &= 0xffffu;
+            bad = true;
           }
         }
+        if (bad) {
+          *at = w;
+          *static_cast<volatile int *>(&sm.dirty) = 1;
+        }
       }
-      fence_async_smem();
-      mbar_arrive(type == 0 ? &sm.q_full : &sm.kv_full[stage]);
-    };
-    auto flush = [&] {
-      if (pending == 0) return;
-      cp_async_wait<0>();
-      finish(pend0);
-      if (pending == 2) finish(pend1);
-      pending = 0;
-    };
-    auto push = [&](uint32_t item) {
-      cp_async_commit();
-      if (pending == 2) {
-        cp_async_wait<2>();
-        finish(pend0);
-        pend0 = pend1;
-        pend1 = item;
-      } else if (pending == 1) {
-        pend1 = item;
-        pending = 2;
-      } else {
-        pend0 = item;
-        pending = 1;
-      }
-    };
-    // Blocks on a barrier only with nothing held back: what is waited for may
-    // need the items still in flight.
-    auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
-      bool got = mbar_try_wait(smem_u32(bar), parity);
-      if (!got) {
-        flush();
-        got = mbar_wait(bar, parity, abort_flag, p.status, kErrTimeoutEmpty);
-      }
-      return __all_sync(0xffffffffu, got) != 0;  // a warp goes on or ends as one
     };
     for (; ok; ++sc) {
       const int ss = sc % SEGS;
@@ -363,7 +331,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
                                  : q;
           cp_async16(smem_u32(sm.q[r >> 7]) + dst0 + (it % PASSES) * STEP * 128, src, live ? 16 : 0);
         }
-        push(0);
+        cp_async_arrive(&sm.q_full);
       }
       // ---- keys and values ----
       const int32_t *table = a.table + sg.b * a.table_stride;
@@ -386,10 +354,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
         const uint32_t bits = __ballot_sync(0xffffffffu, good);
         if (lane == 0) sm.valid[(tiles + j) % VALID_RING][warp] = bits;
         mbar_arrive(&sm.info_ready);
-        // Nothing is held up by items in flight here: every loader gets here
-        // without waiting for anything that this one has not waited for.
-        return __all_sync(0xffffffffu, mbar_wait(&sm.info_ready, described++ & 1, abort_flag,
-                                                 p.status, kErrTimeoutEmpty)) != 0;
+        return wait(&sm.info_ready, described++ & 1);
       };
       auto load = [&](int j, bool value) -> bool {
         const int s = kvc % ST;
@@ -411,8 +376,13 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
           cp_async16(dst + it * STEP * 128, src, row >= 0 ? 16 : 0);
         }
         const int first = min(max(sg.prefix - (key0 + j * BK), 0), BK);
-        push((value && first < BK ? 2u : 1u) | (static_cast<uint32_t>(s) << 2) |
-             (static_cast<uint32_t>(first) << 8));
+        if (value && first < BK) {
+          cp_async_wait_all();
+          clean(sm.kv[s], first);
+          mbar_arrive(&sm.kv_full[s]);
+        } else {
+          cp_async_arrive(&sm.kv_full[s]);
+        }
         return true;
       };
       for (int j = 0; j < AHEAD && j < sg.ntiles && ok; ++j) {
@@ -427,7 +397,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
       tiles += sg.ntiles;
       if (!ok) break;
     }
-    flush();
+    cp_async_wait_all();
   } else if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 12 && lane == 0) {
@@ -447,12 +417,14 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
         const int n = sg.ntiles;
         const int groups = sg.nrows > 128 ? 2 : 1;  // kPair: warpgroups with rows
         if (!mbar_wait(&sm.q_full, sc & 1, abort_flag, p.status, kErrTimeoutFull)) break;
+        fence_async_smem();
         tc_fence_after();
         // Scores of tile j: for both row halves, or for the tile's warpgroup.
         auto scores = [&](int j) -> bool {
           const int s = kvc % ST;
           if (!mbar_wait(&sm.kv_full[s], (kvc / ST) & 1, abort_flag, p.status, kErrTimeoutFull))
             return false;
+          fence_async_smem();
           ++kvc;
           const uint32_t k_addr = smem_u32(sm.kv[s]);
           const int g0 = kPair ? 0 : (j & 1), g1 = kPair ? groups : g0 + 1;
@@ -476,6 +448,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
           const int s = kvc % ST;
           if (!mbar_wait(&sm.kv_full[s], (kvc / ST) & 1, abort_flag, p.status, kErrTimeoutFull))
             return false;
+          fence_async_smem();
           ++kvc;
           const uint32_t v_addr = smem_u32(sm.kv[s]);
           const int g0 = kPair ? 0 : (j & 1), g1 = kPair ? groups : g0 + 1;

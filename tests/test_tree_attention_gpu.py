@@ -97,7 +97,7 @@ SHAPES = [  # new, kv, heads, kv_heads, dim, block
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("tree", [True, False])
 def test_sixteen_bits(mcb, shape, dtype, tree):
-    Case(*shape, dtype, tree).check(mcb)
+    Case(*shape, dtype, tree).check(mcb, "tcgen05_tree_attention")
 
 
 @pytest.mark.parametrize("shape", [
