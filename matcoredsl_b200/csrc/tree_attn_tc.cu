@@ -43,6 +43,7 @@ constexpr int LOADERS = 128;
 constexpr int SEGS = 4;         // ring of segments
 constexpr int VALID_RING = 16;  // key tiles whose validity words are kept
 constexpr int INFO_RING = 4;    // key tiles whose row numbers are kept
+constexpr uint32_t kNoRow = 0xffffffffu;
 constexpr int TMEM_COLS = 512;
 constexpr uint32_t S_COL = 0, O_COL = 256;
 
@@ -72,7 +73,9 @@ struct Smem {
   uint8_t q[kPair ? 2 : 1][tile_bytes<HD>()];
   uint8_t kv[ST][tile_bytes<HD>()];
   uint8_t p[2][128 * BK * 2];
-  int32_t info[INFO_RING][BK];  // cache row of each key of a tile, -1: none
+  // Where a tile's keys lie, block << bits | row, kNoRow: nowhere; ordered so that
+  // a loader's keys lie together.
+  uint32_t info[INFO_RING][BK];
   uint32_t valid[VALID_RING][4];
   Segment seg[SEGS];
   uint64_t seg_full[SEGS], seg_empty[SEGS];
@@ -81,7 +84,8 @@ struct Smem {
   uint64_t s_full[2], s_free[2], p_full[2], p_free[2], o_full[2], o_empty[2];
   uint64_t info_ready, join_full, join_read;
   uint64_t drain;
-  int64_t start_b, start_w;
+  int64_t start_b;
+  int32_t start_w;
   uint32_t tmem_slot;
   int abort_flag, dirty;
 };
@@ -90,12 +94,30 @@ static_assert(sizeof(Smem<128, true>) <= kMaxSmem && sizeof(Smem<128, false>) <=
                   sizeof(Smem<64, true>) <= kMaxSmem && sizeof(Smem<64, false>) <= kMaxSmem,
               "tree attention exceeds the shared memory per block");
 
+// x / d for x < 2^31: x * ceil(2^(31+s) / d) >> (31+s), 2^s >= d > 2^(s-1). The
+// factor is below 2^32 and the error x * (factor * d - 2^(31+s)) below 2^(31+s).
+struct FastDiv {
+  uint32_t mul;
+  int32_t shift;
+};
+__device__ __forceinline__ uint32_t fast_div(uint32_t x, const FastDiv &d) {
+  return static_cast<uint32_t>((static_cast<uint64_t>(x) * d.mul) >> d.shift);
+}
+FastDiv make_div(int32_t d) {
+  int s = 0;
+  while ((static_cast<int64_t>(1) << s) < d) ++s;
+  return {static_cast<uint32_t>(((static_cast<uint64_t>(1) << (31 + s)) + d - 1) /
+                                static_cast<uint64_t>(d)),
+          31 + s};
+}
+
 struct Params {
   TreeAttn a;
   float c;             // |scale| * log2(e)
   uint32_t s_neg;      // negate A in the score product when scale < 0
-  uint32_t div_mul;    // row number / block = row * div_mul >> div_shift (row < 2^31)
-  int32_t div_shift;
+  FastDiv block, group;
+  uint32_t step[2][2];  // block and row strides of K and V in 16 bytes
+  int32_t row_bits;     // bits of a row within a block
   float *partial;      // [2 * CTAs][ROWS][HD] outputs, then [2 * CTAs][ROWS][2] (max, sum)
   TreeAttnPart *part;  // [CTAs]
   uint32_t *status;
@@ -161,10 +183,10 @@ __device__ __forceinline__ int32_t unit_tiles(const TreeAttn &a, const Request &
   return end <= BK ? 1 : static_cast<int32_t>((end + BK - 1) / BK);
 }
 template <int ROWS>
-__device__ __forceinline__ int64_t head_tiles(const TreeAttn &a, const Request &r) {
+__device__ __forceinline__ int32_t head_tiles(const TreeAttn &a, const Request &r) {
   const int32_t rts = (r.rows + ROWS - 1) / ROWS;
-  if (a.mask) return static_cast<int64_t>(rts) * (rts ? unit_tiles<ROWS>(a, r, 0) : 0);
-  int64_t sum = 0;
+  if (a.mask) return rts * (rts ? unit_tiles<ROWS>(a, r, 0) : 0);
+  int32_t sum = 0;
   for (int32_t rt = 0; rt < rts; ++rt) sum += unit_tiles<ROWS>(a, r, rt);
   return sum;
 }
@@ -193,7 +215,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
   constexpr int AHEAD = kPair ? 1 : 2;  // score tiles issued before the first value tile
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem<HD, kPair> &sm = *reinterpret_cast<Smem<HD, kPair> *>(smem_raw);
-  int64_t *scan = reinterpret_cast<int64_t *>(sm.info);  // before the roles start
+  int32_t *scan = reinterpret_cast<int32_t *>(sm.info);  // before the roles start
   const TreeAttn &a = p.a;
   volatile int *abort_flag = &sm.abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -237,13 +259,13 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
   const int64_t per_thread = (a.requests + THREADS - 1) / THREADS;
   const int64_t b_first = threadIdx.x * per_thread;
   const int64_t b_last = min(a.requests, b_first + per_thread);
-  int64_t mine = 0;
+  int32_t mine = 0;
   for (int64_t b = b_first; b < b_last; ++b)
     mine += head_tiles<ROWS>(a, load_request(a, b)) * a.kv_heads;
-  int64_t incl = mine;
+  int32_t incl = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const int64_t o = __shfl_up_sync(0xffffffffu, incl, off);
+    const int32_t o = __shfl_up_sync(0xffffffffu, incl, off);
     if (lane >= off) incl += o;
   }
   if (lane == 31) scan[warp] = incl;
@@ -251,15 +273,18 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem_slot;
-  int64_t total = 0, before = incl - mine;
+  int32_t total = 0, before = incl - mine;
+#pragma unroll
   for (int w = 0; w < THREADS / 32; ++w) {
     if (w < warp) before += scan[w];
     total += scan[w];
   }
-  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total);
-  const bool works = blockIdx.x < ctas && !sm.abort_flag;
-  const int64_t w0 = works ? blockIdx.x * total / ctas : 0;
-  const int64_t w1 = works ? (blockIdx.x + 1) * total / ctas : 0;
+  // The first `extra` CTAs take share + 1 tiles, the others share.
+  const int32_t cta = blockIdx.x, ctas = min(static_cast<int32_t>(gridDim.x), total);
+  const bool works = cta < ctas && !sm.abort_flag;
+  const int32_t share = works ? total / ctas : 0, extra = works ? total - share * ctas : 0;
+  const int32_t w0 = cta * share + min(cta, extra);
+  const int32_t w1 = works ? w0 + share + (cta < extra) : w0;
   // The thread whose requests hold tile w0 leaves where they begin.
   if (works && before <= w0 && w0 < before + mine) {
     sm.start_b = b_first;
@@ -320,16 +345,16 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
       // ---- queries ----
       if (!(ok = wait(&sm.q_empty, (sc & 1) ^ 1))) break;
       {
-        const char *q = static_cast<const char *>(a.q) + piece * 16;
-        for (int it = 0; it < PASSES * (kPair ? 2 : 1); ++it) {
-          const int r = r0 + it * STEP;
-          const int row = sg.row0 + r, tok = row / group;
-          const bool live = r < sg.nrows;
-          const char *src = live ? q + ((static_cast<int64_t>(sg.tok0) + tok) * a.q_s[0] +
-                                        (static_cast<int64_t>(sg.head) * group + row - tok * group) *
-                                            a.q_s[1]) * 2
-                                 : q;
-          cp_async16(smem_u32(sm.q[r >> 7]) + dst0 + (it % PASSES) * STEP * 128, src, live ? 16 : 0);
+        // Rows past the last one keep what they held: a row of a product depends
+        // on no other row.
+        const char *q = static_cast<const char *>(a.q) +
+                        (sg.tok0 * a.q_s[0] + sg.head * group * a.q_s[1] + piece * 8) * 2;
+#pragma unroll 4
+        for (int r = r0; r < sg.nrows; r += STEP) {
+          const int row = sg.row0 + r, tok = fast_div(row, p.group);
+          cp_async16(smem_u32(sm.q[0]) + (r >> 7) * tile_bytes<HD>() + dst0 +
+                         ((r & 127) - r0) * 128,
+                     q + (tok * a.q_s[0] + (row - tok * group) * a.q_s[1]) * 2, 16);
         }
         cp_async_arrive(&sm.q_full);
       }
@@ -339,18 +364,18 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
       auto entry = [&](int j) -> int32_t {  // block of this thread's key of tile j
         const int key = key0 + j * BK + l;
         if (j >= sg.ntiles || key >= sg.keys) return -1;
-        return table[static_cast<uint32_t>(
-            (static_cast<uint64_t>(key) * p.div_mul) >> p.div_shift)];
+        return table[fast_div(key, p.block)];
       };
       int32_t next = entry(0);
       auto describe = [&](int j) -> bool {
         const int key = key0 + j * BK + l;
         const int32_t blk = next;
         next = entry(j + 1);
-        const uint32_t col = static_cast<uint32_t>(
-            (static_cast<uint64_t>(key) * p.div_mul) >> p.div_shift);
         const bool good = key < sg.keys && blk >= 0 && blk < a.blocks;
-        sm.info[j % INFO_RING][l] = good ? blk * a.block + (key - static_cast<int>(col) * a.block) : -1;
+        const uint32_t col = fast_div(key, p.block);
+        const uint32_t off = key - col * a.block;
+        sm.info[j % INFO_RING][(l % STEP) * PASSES + l / STEP] =
+            good ? (static_cast<uint32_t>(blk) << p.row_bits) | off : kNoRow;
         const uint32_t bits = __ballot_sync(0xffffffffu, good);
         if (lane == 0) sm.valid[(tiles + j) % VALID_RING][warp] = bits;
         mbar_arrive(&sm.info_ready);
@@ -360,20 +385,24 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
         const int s = kvc % ST;
         if (!wait(&sm.kv_empty[s], ((kvc / ST) & 1) ^ 1)) return false;
         ++kvc;
-        const int64_t *st = value ? a.v_s : a.k_s;
-        const char *base = static_cast<const char *>(value ? a.v : a.k) + sg.head * st[2] * 2 +
-                           piece * 16;
+        const char *base = static_cast<const char *>(value ? a.v : a.k) +
+                           (sg.head * (value ? a.v_s[2] : a.k_s[2]) + piece * 8) * 2;
         const uint32_t dst = smem_u32(sm.kv[s]) + dst0;
+        const uint32_t blk_step = p.step[value][0], row_step = p.step[value][1];
+        const uint4 *info =
+            reinterpret_cast<const uint4 *>(sm.info[j % INFO_RING]) + r0 * (PASSES / 4);
 #pragma unroll
-        for (int it = 0; it < PASSES; ++it) {
-          const int32_t row = sm.info[j % INFO_RING][r0 + it * STEP];
-          const char *src = base;
-          if (row >= 0) {
-            const uint32_t blk = static_cast<uint32_t>(
-                (static_cast<uint64_t>(row) * p.div_mul) >> p.div_shift);
-            src += (blk * st[0] + (row - static_cast<int32_t>(blk) * a.block) * st[1]) * 2;
+        for (int it = 0; it < PASSES; it += 4) {
+          const uint4 w = info[it / 4];
+          const uint32_t row[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const bool none = row[u] == kNoRow;
+            const uint32_t at = (row[u] >> p.row_bits) * blk_step +
+                                (row[u] & ((1u << p.row_bits) - 1)) * row_step;
+            cp_async16(dst + (it + u) * STEP * 128,
+                       base + static_cast<uint64_t>(none ? 0u : at) * 16, none ? 0 : 16);
           }
-          cp_async16(dst + it * STEP * 128, src, row >= 0 ? 16 : 0);
         }
         const int first = min(max(sg.prefix - (key0 + j * BK), 0), BK);
         if (value && first < BK) {
@@ -405,7 +434,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
       constexpr uint32_t F = kF16 ? 0 : 1;
       const uint32_t idesc_s = make_idesc(F, F, 0, 0, 128, BK) | p.s_neg;
       const uint32_t idesc_o = make_idesc(F, F, 0, 1, 128, HD);
-      uint32_t kvc = 0, sc = 0, s_cnt[2] = {0, 0}, p_cnt[2] = {0, 0}, o_cnt[2] = {0, 0};
+      // Bit g: parity of warpgroup g's phase. (Counters indexed by g would live in
+      // local memory, whose loads queue behind the loaders' copies.)
+      uint32_t kvc = 0, sc = 0, s_par = 0, p_par = 0, o_par = 0;
       bool ok = true;
       for (; ok; ++sc) {
         const int ss = sc % SEGS;
@@ -429,10 +460,10 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
           const uint32_t k_addr = smem_u32(sm.kv[s]);
           const int g0 = kPair ? 0 : (j & 1), g1 = kPair ? groups : g0 + 1;
           for (int g = g0; g < g1; ++g) {
-            if (!mbar_wait(&sm.s_free[g], (s_cnt[g] & 1) ^ 1, abort_flag, p.status,
+            if (!mbar_wait(&sm.s_free[g], ((s_par >> g) & 1) ^ 1, abort_flag, p.status,
                            kErrTimeoutAccum))
               return false;
-            ++s_cnt[g];
+            s_par ^= 1u << g;
             tc_fence_after();
             const uint32_t q_addr = smem_u32(sm.q[kPair ? g : 0]);
 #pragma unroll
@@ -456,14 +487,14 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
             const bool first = kPair ? j == 0 : j < 2;
             const bool last = kPair ? j + 1 == n : j + 2 >= n;
             if (first) {
-              if (!mbar_wait(&sm.o_empty[g], (o_cnt[g] & 1) ^ 1, abort_flag, p.status,
+              if (!mbar_wait(&sm.o_empty[g], ((o_par >> g) & 1) ^ 1, abort_flag, p.status,
                              kErrTimeoutAccum))
                 return false;
-              ++o_cnt[g];
+              o_par ^= 1u << g;
             }
-            if (!mbar_wait(&sm.p_full[g], p_cnt[g] & 1, abort_flag, p.status, kErrTimeoutAccum))
+            if (!mbar_wait(&sm.p_full[g], (p_par >> g) & 1, abort_flag, p.status, kErrTimeoutAccum))
               return false;
-            ++p_cnt[g];
+            p_par ^= 1u << g;
             tc_fence_after();
             const uint32_t p_addr = smem_u32(sm.p[g]);
 #pragma unroll
@@ -504,24 +535,25 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
         return true;
       };
       if (w0 < w1) {
-        int64_t w = w0, b = sm.start_b, at = sm.start_w;  // `at`: first tile of request b
+        int64_t b = sm.start_b;
+        int32_t w = w0, at = sm.start_w;  // `at`: first tile of request b
         Request r = load_request(a, b);
-        int64_t per = head_tiles<ROWS>(a, r);
+        int32_t per = head_tiles<ROWS>(a, r);
         while (at + per * a.kv_heads <= w) {
           at += per * a.kv_heads;
           r = load_request(a, ++b);
           per = head_tiles<ROWS>(a, r);
         }
-        int32_t head = static_cast<int32_t>((w - at) / per), rt = 0;
-        int64_t rest = w - at - head * per;
+        int32_t head = (w - at) / per, rt = 0;
+        int32_t rest = w - at - head * per;
         int32_t n = unit_tiles<ROWS>(a, r, 0);
         while (rest >= n) {
           rest -= n;
           n = unit_tiles<ROWS>(a, r, ++rt);
         }
-        int32_t tile0 = static_cast<int32_t>(rest);
+        int32_t tile0 = rest;
         while (ok) {
-          const int32_t take = static_cast<int32_t>(min(static_cast<int64_t>(n - tile0), w1 - w));
+          const int32_t take = min(n - tile0, w1 - w);
           const bool ends = tile0 + take == n;
           Segment sg;
           sg.kind = tile0 > 0 ? kHead : ends ? kWhole : kTail;
@@ -537,8 +569,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
           sg.ntiles = take;
           if (sg.kind == kTail) {
             // Last CTA with a part of this unit.
-            const int64_t last = w - tile0 + n - 1;
-            part.parts = static_cast<int32_t>(((last + 1) * ctas - 1) / total - blockIdx.x) + 1;
+            const int32_t last = w - tile0 + n - 1, big = extra * (share + 1);
+            part.parts = (last < big ? last / (share + 1) : extra + (last - big) / share) - cta + 1;
             part.tok0 = r.tok0;
             part.head = head;
             part.row0 = sg.row0;
@@ -575,7 +607,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
     const uint32_t s_col = S_COL + g * BK, o_col = O_COL + g * HD;
     uint8_t *p_row = sm.p[g] + row * 128;
     const int rsw = row & 7;
-    uint32_t sc = 0, s_cnt = 0, p_cnt = 0, o_cnt[2] = {0, 0}, tiles = 0, joins = 0;
+    uint32_t sc = 0, s_cnt = 0, p_cnt = 0, o_cnt = 0, tiles = 0, joins = 0;
     bool ok = true;
     for (; ok; ++sc) {
       const int ss = sc % SEGS;
@@ -592,7 +624,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
       const bool busy = kPair ? base < sg.nrows : g < n;
       const bool live = base + sub * 32 < sg.nrows;  // this warp has rows
       const int urow = min(sg.row0 + base + row, sg.row0 + sg.nrows - 1);
-      const int i = urow / group;                    // new token of this row
+      const int i = fast_div(urow, p.group);         // new token of this row
       const uint32_t *mask_row =
           a.mask ? a.mask + (static_cast<int64_t>(sg.tok0) + i) * a.mask_stride : nullptr;
       float m_ref = -INFINITY, l = 0.0f;
@@ -718,14 +750,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
       if (!busy) continue;
       float mc = m_ref == -INFINITY ? -INFINITY : m_ref * p.c;
       float w_own = 1.0f, w_other = 0.0f;
-      for (int h = 0; h < 2; ++h) {
-        if (h != g && !(joined && g == 0)) continue;
-        if (!(ok = mbar_wait_warp(&sm.o_full[h], o_cnt[h] & 1, abort_flag, p.status,
-                                  kErrTimeoutAccum)))
-          break;
-        ++o_cnt[h];
-      }
-      if (!ok) break;
+      if (!(ok = mbar_wait_warp(&sm.o_full[g], o_cnt++ & 1, abort_flag, p.status,
+                                kErrTimeoutAccum)))
+        break;
+      if (joined && g == 0 &&
+          !(ok = mbar_wait_warp(&sm.o_full[1], joins & 1, abort_flag, p.status, kErrTimeoutAccum)))
+        break;
       tc_fence_after();
       if (joined) {
         // Warpgroup 1 leaves its maximum and sum in its weights' buffer (free
@@ -935,8 +965,20 @@ bool tree_attn_tc_ok(const TreeAttn &a, int dtype) {
                           reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.o);
   int64_t steps = a.q_s[0] | a.q_s[1] | a.o_s[0] | a.o_s[1];
   for (int i = 0; i < 3; ++i) steps |= a.k_s[i] | a.v_s[i];
-  return bases % 16 == 0 && steps % 8 == 0 && a.tokens * a.heads <= 0x7fffffff &&
-         a.columns * a.block <= 0x7fffff00;
+  if (bases % 16 != 0 || steps % 8 != 0) return false;
+  // 32-bit numbers: rows, keys of a request, all key tiles, and the offsets of
+  // cache rows in 16 bytes (a cache of up to 64 GB).
+  const int64_t group = a.heads / a.kv_heads, rows = a.tokens * group;
+  if (a.tokens * a.heads > 0x7fffffff || a.columns * a.block > 0x7fffff00) return false;
+  const double tiles = (static_cast<double>(rows) / 128 + a.requests) * a.kv_heads *
+                       (static_cast<double>(a.columns) * a.block / BK + 1);
+  if (tiles > 0x7fffffff) return false;
+  for (const int64_t *st : {a.k_s, a.v_s})
+    if (st[0] / 8 > 0xffffffffLL || st[1] / 8 > 0xffffffffLL ||
+        static_cast<double>(a.blocks) * (st[0] / 8) + static_cast<double>(a.block) * (st[1] / 8) >=
+            4294967295.0)
+      return false;
+  return true;
 }
 
 uint64_t tree_attn_tc_scratch(const TreeAttn &a, int sms) {
@@ -951,12 +993,13 @@ cudaError_t launch_tree_attn_tc(const TreeAttn &a, int dtype, void *scratch, uin
   p.a = a;
   p.c = fabsf(a.scale) * 1.4426950408889634f;
   p.s_neg = a.scale < 0.0f ? kIdescNegateA : 0u;
-  // x / d for x < 2^31: x * ceil(2^(31+s) / d) >> (31+s) with 2^s >= d.
-  int s = 0;
-  while ((static_cast<int64_t>(1) << s) < a.block) ++s;
-  p.div_shift = 31 + s;
-  p.div_mul = static_cast<uint32_t>(
-      ((static_cast<uint64_t>(1) << (31 + s)) + a.block - 1) / static_cast<uint64_t>(a.block));
+  p.block = make_div(a.block);
+  p.group = make_div(a.heads / a.kv_heads);
+  for (int i = 0; i < 2; ++i) {
+    p.step[0][i] = static_cast<uint32_t>(a.k_s[i] / 8);
+    p.step[1][i] = static_cast<uint32_t>(a.v_s[i] / 8);
+  }
+  p.row_bits = p.block.shift - 31;  // blocks * block < 2^31, so block << bits | row < 2^32 - 1
   p.partial = static_cast<float *>(scratch);
   p.part = reinterpret_cast<TreeAttnPart *>(
       p.partial + static_cast<uint64_t>(sms) * 2 * (pair ? 256 : 128) * (a.dim + 2));
