@@ -47,9 +47,10 @@ SOURCES = {
     "rope.cu": [],
     "tree_attn.cu": [],
     "tree_attn_tc.cu": [],
+    "tree_attn_few.cu": [],
     "logits.cu": [],
 }
-HEADERS = ["common.cuh", "internal.h", "epilogue.cuh"]
+HEADERS = ["common.cuh", "internal.h", "epilogue.cuh", "tree_attn.cuh"]
 
 
 def _newer(src_paths, out):

@@ -2275,16 +2275,22 @@ mcb_status tree_attention_impl(const mcb_tensor *o, const mcb_tensor *lse, const
   LaunchInfo info;
   void *scratch = nullptr;
   const int dt = static_cast<int>(q->dtype);
-  const bool tc = mcb::tree_attn_tc_ok(p, dt);
-  const uint64_t bytes = tc ? mcb::tree_attn_tc_scratch(p, call.sms())
-                            : mcb::tree_attn_simt_scratch(p, call.sms());
+  const bool few = mcb::tree_attn_few_ok(p, dt), tc = !few && mcb::tree_attn_tc_ok(p, dt);
+  const uint64_t bytes = few  ? mcb::tree_attn_few_scratch(p, call.sms())
+                         : tc ? mcb::tree_attn_tc_scratch(p, call.sms())
+                              : mcb::tree_attn_simt_scratch(p, call.sms());
   if (bytes && (s = call.scratch(bytes, &scratch))) return s;
   call.mark_compute_start();
-  const cudaError_t err =
-      tc ? mcb::launch_tree_attn_tc(p, dt, scratch, call.ctx()->status, call.sms(), call.stream(),
-                                    &info)
-         : mcb::launch_tree_attn_simt(p, dt, static_cast<float *>(scratch), call.sms(),
-                                      call.stream(), &info);
+  cudaError_t err;
+  if (few)
+    err = mcb::launch_tree_attn_few(p, dt, scratch, call.ctx()->status, call.sms(), call.stream(),
+                                    &info);
+  else if (tc)
+    err = mcb::launch_tree_attn_tc(p, dt, scratch, call.ctx()->status, call.sms(), call.stream(),
+                                   &info);
+  else
+    err = mcb::launch_tree_attn_simt(p, dt, static_cast<float *>(scratch), call.sms(),
+                                     call.stream(), &info);
   call.mark_compute_end();
   if (err == cudaErrorNotSupported) return MCB_STATUS_UNAVAILABLE_VARIANT;
   return call.finish(nullptr, nullptr, info, err);

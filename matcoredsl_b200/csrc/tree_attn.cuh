@@ -1,0 +1,359 @@
+// Shared by the tensor-core kernels of the attention over a paged cache
+// (tree_attn_tc.cu, tree_attn_few.cu): how units of rows and their key tiles are
+// shared out over the CTAs, which keys a row sees, and the launch that joins the
+// parts of a unit.
+//
+// A unit is one request, one key head and up to ROWS of the request's rows
+// (row = new token x query heads of the group); its keys are cut into tiles of
+// 128. Every CTA takes an equal share of all units' tiles, in order, so a long
+// context is split over many CTAs and many short ones are packed into one. The
+// share is found on the device from the lengths: nothing is read by the host. A
+// unit that lies in one CTA is finished there; the parts of a unit that spans
+// CTAs go to scratch (at most two per CTA) and a second launch joins them in
+// their order.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "internal.h"
+
+namespace mcb {
+namespace tree {
+
+constexpr int BK = 128;  // keys per tile
+constexpr uint32_t kNoRow = 0xffffffffu;
+
+// A CTA's part of a unit.
+struct Segment {
+  int32_t kind;          // kWhole, kHead, kTail, or kEnd
+  int32_t b, head;       // request, key head
+  int32_t row0, nrows;   // rows of the request
+  int32_t tok0;          // first new token
+  int32_t prefix, keys;  // position of the first new token; keys there are
+  int32_t tile0, ntiles;
+};
+enum : int32_t { kEnd = -1, kWhole = 0, kHead = 1, kTail = 2 };
+
+// x / d for x < 2^31: x * ceil(2^(31+s) / d) >> (31+s), 2^s >= d > 2^(s-1). The
+// factor is below 2^32 and the error x * (factor * d - 2^(31+s)) below 2^(31+s).
+struct FastDiv {
+  uint32_t mul;
+  int32_t shift;
+};
+__device__ __forceinline__ uint32_t fast_div(uint32_t x, const FastDiv &d) {
+  return static_cast<uint32_t>((static_cast<uint64_t>(x) * d.mul) >> d.shift);
+}
+inline FastDiv make_div(int32_t d) {
+  int s = 0;
+  while ((static_cast<int64_t>(1) << s) < d) ++s;
+  return {static_cast<uint32_t>(((static_cast<uint64_t>(1) << (31 + s)) + d - 1) /
+                                static_cast<uint64_t>(d)),
+          31 + s};
+}
+
+struct TreeParams {
+  TreeAttn a;
+  float c;             // |scale| * log2(e)
+  FastDiv block, group;
+  uint32_t step[2][2];  // block and row strides of K and V in 16 bytes
+  int32_t row_bits;     // bits of a row within a block
+  float *partial;      // [2 * CTAs][ROWS][HD] outputs, then [2 * CTAs][ROWS][2] (max, sum)
+  TreeAttnPart *part;  // [CTAs]
+  uint32_t *status;
+};
+
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <bool kF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  return kF16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
+}
+// 16 bytes to shared memory, zeros when `bytes` is 0.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(bytes)
+               : "memory");
+}
+// One arrival on `bar` once this thread's copies so far have landed. The
+// copies are generic-proxy writes: whoever waits on the barrier fences before a
+// tensor-core instruction reads them.
+__device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// One request's lengths, clipped to the tensors.
+struct Request {
+  int32_t tok0, n, rows, prefix, keys;  // rows: of the tokens inside [0, T)
+};
+__device__ __forceinline__ Request load_request(const TreeAttn &a, int64_t b) {
+  Request r;
+  const int64_t c0 = a.cu[b], c1 = a.cu[b + 1], kv = max(0, a.kv_lens[b]);
+  const int64_t n = c0 >= 0 && c1 > c0 ? c1 - c0 : 0;
+  const int64_t in = max(static_cast<int64_t>(0), min(n, a.tokens - c0));
+  r.tok0 = static_cast<int32_t>(c0);
+  r.n = static_cast<int32_t>(n);
+  r.rows = static_cast<int32_t>(in * (a.heads / a.kv_heads));
+  r.prefix = static_cast<int32_t>(kv - n);
+  r.keys = static_cast<int32_t>(min(kv, a.columns * a.block));
+  return r;
+}
+// Key tiles of row tile `rt`: without a mask the rows see no key past the
+// last one's own.
+template <int ROWS>
+__device__ __forceinline__ int32_t unit_tiles(const TreeAttn &a, const Request &r, int32_t rt) {
+  int64_t end = r.keys;
+  if (!a.mask) {
+    const int32_t last = min(r.rows, (rt + 1) * ROWS) - 1;
+    end = min(end, static_cast<int64_t>(r.prefix) + last / (a.heads / a.kv_heads) + 1);
+  }
+  return end <= BK ? 1 : static_cast<int32_t>((end + BK - 1) / BK);
+}
+template <int ROWS>
+__device__ __forceinline__ int32_t head_tiles(const TreeAttn &a, const Request &r) {
+  const int32_t rts = (r.rows + ROWS - 1) / ROWS;
+  if (a.mask) return rts * (rts ? unit_tiles<ROWS>(a, r, 0) : 0);
+  int32_t sum = 0;
+  for (int32_t rt = 0; rt < rts; ++rt) sum += unit_tiles<ROWS>(a, r, rt);
+  return sum;
+}
+
+// Bits of the 32 keys from position pos on that new token i (mask row `row`)
+// may see; bit k is key pos + k.
+__device__ __forceinline__ uint32_t visible_word(const TreeAttn &a, const uint32_t *row,
+                                                 int32_t pos, int32_t prefix, int32_t i) {
+  const int64_t j = static_cast<int64_t>(pos) - prefix;  // new token of bit 0
+  if (j <= -32) return 0xffffffffu;
+  if (!row) {
+    const int64_t n = static_cast<int64_t>(i) - j + 1;  // keys up to the token itself
+    return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1;
+  }
+  auto word = [&](int64_t w) -> uint32_t { return w >= 0 && w < a.mask_words ? row[w] : 0u; };
+  if (j < 0) return (word(0) << -j) | ((1u << -j) - 1);
+  const int32_t s = static_cast<int32_t>(j & 31);
+  const uint32_t lo = word(j >> 5);
+  return s ? (lo >> s) | (word((j >> 5) + 1) << (32 - s)) : lo;
+}
+
+// This CTA's share [w0, w1) of all tiles, found by all THREADS threads of it
+// (`scan`: THREADS / 32 words of shared memory), and where the requests that hold
+// tile w0 begin. The first `extra` CTAs take share + 1 tiles, the others share.
+struct Share {
+  int32_t w0, w1, share, extra;
+};
+template <int ROWS, int THREADS>
+__device__ __forceinline__ Share find_share(const TreeAttn &a, int32_t *scan, bool usable,
+                                            int64_t *start_b, int32_t *start_w) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t per_thread = (a.requests + THREADS - 1) / THREADS;
+  const int64_t b_first = threadIdx.x * per_thread;
+  const int64_t b_last = min(a.requests, b_first + per_thread);
+  int32_t mine = 0;
+  for (int64_t b = b_first; b < b_last; ++b)
+    mine += head_tiles<ROWS>(a, load_request(a, b)) * a.kv_heads;
+  int32_t incl = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int32_t o = __shfl_up_sync(0xffffffffu, incl, off);
+    if (lane >= off) incl += o;
+  }
+  if (lane == 31) scan[warp] = incl;
+  __syncthreads();
+  int32_t total = 0, before = incl - mine;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += scan[w];
+    total += scan[w];
+  }
+  const int32_t cta = blockIdx.x, ctas = min(static_cast<int32_t>(gridDim.x), total);
+  const bool works = cta < ctas && usable;
+  Share s;
+  s.share = works ? total / ctas : 0;
+  s.extra = works ? total - s.share * ctas : 0;
+  s.w0 = cta * s.share + min(cta, s.extra);
+  s.w1 = works ? s.w0 + s.share + (cta < s.extra) : s.w0;
+  // The thread whose requests hold tile w0 leaves where they begin.
+  if (works && before <= s.w0 && s.w0 < before + mine) {
+    *start_b = b_first;
+    *start_w = before;
+  }
+  __syncthreads();
+  return s;
+}
+
+// One thread's walk over the segments of a share.
+template <int ROWS>
+struct Walk {
+  const TreeAttn &a;
+  const Share &sh;
+  TreeAttnPart &part;  // the unit that starts in this CTA and ends in a later one
+  Request r;
+  int64_t b;
+  int32_t w, head = 0, rt = 0, n = 0, tile0 = 0;
+
+  __device__ __forceinline__ Walk(const TreeAttn &args, const Share &share, TreeAttnPart &p,
+                                  int64_t start_b, int32_t start_w)
+      : a(args), sh(share), part(p), b(start_b), w(share.w0) {
+    if (w >= sh.w1) return;
+    int32_t at = start_w;  // first tile of request b
+    r = load_request(a, b);
+    int32_t per = head_tiles<ROWS>(a, r);
+    while (at + per * a.kv_heads <= w) {
+      at += per * a.kv_heads;
+      r = load_request(a, ++b);
+      per = head_tiles<ROWS>(a, r);
+    }
+    head = (w - at) / per;
+    tile0 = w - at - head * per;
+    n = unit_tiles<ROWS>(a, r, 0);
+    while (tile0 >= n) {
+      tile0 -= n;
+      n = unit_tiles<ROWS>(a, r, ++rt);
+    }
+  }
+  // False past the last segment.
+  __device__ __forceinline__ bool next(Segment &sg) {
+    if (w >= sh.w1) return false;
+    if (n == 0) {  // a new unit
+      if ((rt + 1) * ROWS < r.rows) {
+        ++rt;
+      } else {
+        rt = 0;
+        if (++head == a.kv_heads) {
+          head = 0;
+          do r = load_request(a, ++b);
+          while (r.rows == 0);
+        }
+      }
+      n = unit_tiles<ROWS>(a, r, rt);
+      tile0 = 0;
+    }
+    const int32_t take = min(n - tile0, sh.w1 - w);
+    sg.kind = tile0 > 0 ? kHead : take == n ? kWhole : kTail;
+    sg.b = static_cast<int32_t>(b);
+    sg.head = head;
+    sg.row0 = rt * ROWS;
+    sg.nrows = min(r.rows - sg.row0, ROWS);
+    sg.tok0 = r.tok0;
+    sg.prefix = r.prefix;
+    sg.keys = r.keys;
+    sg.tile0 = tile0;
+    sg.ntiles = take;
+    if (sg.kind == kTail) {
+      const int32_t last = w + n - 1, big = sh.extra * (sh.share + 1);  // the unit's last tile
+      part.parts = (last < big ? last / (sh.share + 1) : sh.extra + (last - big) / sh.share) -
+                   static_cast<int32_t>(blockIdx.x) + 1;
+      part.tok0 = r.tok0;
+      part.head = head;
+      part.row0 = sg.row0;
+      part.nrows = sg.nrows;
+    }
+    w += take;
+    n = 0;
+    return true;
+  }
+};
+
+// Joins the parts of the units that span CTAs, in their order, one warp a row;
+// the last column of CTAs clears the tokens of no request.
+template <int HD, int ROWS, bool kF16>
+__global__ void __launch_bounds__(256) tree_attn_join_parts_kernel(const TreeParams p, int ctas) {
+  const TreeAttn &a = p.a;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int group = a.heads / a.kv_heads;
+  if (blockIdx.x == ctas) {
+    const int64_t c0 = min(max(static_cast<int64_t>(a.cu[0]), static_cast<int64_t>(0)), a.tokens);
+    const int64_t c1 = max(c0, min(static_cast<int64_t>(a.cu[a.requests]), a.tokens));
+    const int64_t none = c0 + a.tokens - c1;  // tokens before the first and after the last request
+    for (int64_t w = blockIdx.y * 8 + warp; w < none * a.heads; w += 8 * gridDim.y) {
+      const int64_t at = w / a.heads, h = w - at * a.heads, t = at < c0 ? at : at - c0 + c1;
+      uint32_t *o = reinterpret_cast<uint32_t *>(static_cast<char *>(a.o) +
+                                                 (t * a.o_s[0] + h * a.o_s[1]) * 2);
+      for (int d = lane; d < HD / 2; d += 32) o[d] = 0;
+      if (lane == 0 && a.lse) a.lse[t * a.lse_s + h] = -INFINITY;
+    }
+    return;
+  }
+  const TreeAttnPart part = p.part[blockIdx.x];
+  if (part.parts == 0) return;
+  const float2 *ml = reinterpret_cast<const float2 *>(p.partial +
+                                                      static_cast<int64_t>(ctas) * 2 * ROWS * HD);
+  // Part k: the tail slot of this CTA, then the head slots of the next ones.
+  auto slot = [&](int k) -> int64_t {
+    return (static_cast<int64_t>(blockIdx.x) + k) * 2 + (k == 0);
+  };
+  constexpr int V = HD / 32;
+  for (int r = blockIdx.y * 8 + warp; r < part.nrows; r += 8 * gridDim.y) {
+    float top = -INFINITY;
+    for (int k = lane; k < part.parts; k += 32) top = fmaxf(top, ml[slot(k) * ROWS + r].x);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float l = 0.0f, x[V] = {};
+#pragma unroll 4
+    for (int k = 0; k < part.parts; ++k) {
+      const float2 z = ml[slot(k) * ROWS + r];
+      const float w = ex2(z.x - ref);
+      l += z.y * w;
+      const float *in = p.partial + (slot(k) * ROWS + r) * HD + lane * V;
+      float y[V];
+      if (V == 4) {
+        const float4 f = *reinterpret_cast<const float4 *>(in);
+        y[0] = f.x, y[1] = f.y, y[V - 2] = f.z, y[V - 1] = f.w;
+      } else {
+        const float2 f = *reinterpret_cast<const float2 *>(in);
+        y[0] = f.x, y[1] = f.y;
+      }
+#pragma unroll
+      for (int d = 0; d < V; ++d) x[d] = fmaf(y[d], w, x[d]);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int row = part.row0 + r, i = row / group;
+    const int64_t tok = static_cast<int64_t>(part.tok0) + i;
+    const int head = part.head * group + row - i * group;
+    uint32_t *o = reinterpret_cast<uint32_t *>(static_cast<char *>(a.o) +
+                                               (tok * a.o_s[0] + head * a.o_s[1]) * 2);
+#pragma unroll
+    for (int d = 0; d < V / 2; ++d)
+      o[lane * (V / 2) + d] = pack2<kF16>(x[2 * d] * inv, x[2 * d + 1] * inv);
+    if (lane == 0 && a.lse)
+      a.lse[tok * a.lse_s + head] =
+          l == 0.0f ? -INFINITY : (ref + log2f(l)) * 0.69314718055994531f;
+  }
+}
+
+// The arguments that both kernels take.
+inline TreeParams tree_params(const TreeAttn &a, void *scratch, int rows, int ctas,
+                              uint32_t *status) {
+  TreeParams p;
+  p.a = a;
+  p.c = fabsf(a.scale) * 1.4426950408889634f;
+  p.block = make_div(a.block);
+  p.group = make_div(a.heads / a.kv_heads);
+  for (int i = 0; i < 2; ++i) {
+    p.step[0][i] = static_cast<uint32_t>(a.k_s[i] / 8);
+    p.step[1][i] = static_cast<uint32_t>(a.v_s[i] / 8);
+  }
+  p.row_bits = p.block.shift - 31;  // blocks * block < 2^31, so block << bits | row < 2^32 - 1
+  p.partial = static_cast<float *>(scratch);
+  p.part = reinterpret_cast<TreeAttnPart *>(p.partial +
+                                            static_cast<uint64_t>(ctas) * 2 * rows * (a.dim + 2));
+  p.status = status;
+  return p;
+}
+inline uint64_t tree_scratch(const TreeAttn &a, int rows, int ctas) {
+  return static_cast<uint64_t>(ctas) *
+         (2ull * rows * (a.dim + 2) * sizeof(float) + sizeof(TreeAttnPart));
+}
+
+}  // namespace tree
+}  // namespace mcb
