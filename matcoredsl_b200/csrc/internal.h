@@ -313,7 +313,7 @@ cudaError_t launch_tree_attn_tc(const TreeAttn &p, int dtype, void *scratch, uin
                                 int sms, cudaStream_t stream, LaunchInfo *info);
 
 // ---- tree_attn_few.cu: the same for requests of few rows --------------------------------------
-constexpr int64_t kTreeFewRows = 64;  // rows (new tokens x group) of a request, on average
+constexpr int64_t kTreeFewRows = 32;  // rows (new tokens x group) of a request, on average
 bool tree_attn_few_ok(const TreeAttn &p, int dtype);
 uint64_t tree_attn_few_scratch(const TreeAttn &p, int sms);
 cudaError_t launch_tree_attn_few(const TreeAttn &p, int dtype, void *scratch, uint32_t *status,
@@ -340,6 +340,11 @@ bool encode_tmap_2d(CUtensorMap *map, CUtensorMapDataType dtype, const void *bas
 bool encode_tmap_3d(CUtensorMap *map, CUtensorMapDataType dtype, const void *base,
                     uint64_t d0, uint64_t d1, uint64_t d2, uint64_t stride1_bytes,
                     uint64_t stride2_bytes, uint32_t box0, uint32_t box1, uint32_t box2,
+                    CUtensorMapSwizzle swizzle);
+// dims from the innermost on; byte strides of dims 1..3 (those of a dim of
+// extent 1 are ignored).
+bool encode_tmap_4d(CUtensorMap *map, CUtensorMapDataType dtype, const void *base,
+                    const uint64_t *dims, const uint64_t *strides, const uint32_t *box,
                     CUtensorMapSwizzle swizzle);
 
 }  // namespace mcb

@@ -1,27 +1,32 @@
 // Attention of drafted tokens over a paged cache for requests of few rows (a
-// row = new token x query heads of the group), up to about 64: bf16 or f16,
+// row = new token x query heads of the group), up to 32: bf16 or f16,
 // head size 64 or 128, 16-byte aligned rows. (The mathematics and the masks:
 // tree_attn.cu; how the work is shared out: tree_attn.cuh.)
 //
 // Bound: reading the cache. With R rows a key and value row of 4 * HD bytes
 // take 4 * HD * R operations, far below what a CTA can do in the time of the
-// read, so the kernel is built around the copies: at any time three to four
-// half tiles (128 keys or values, 32 KiB at HD = 128) are on their way to
-// shared memory. The products use warp-level matrix instructions on 16-row tiles:
-// the 128-row tile of a tcgen05 instruction would be empty but for a few rows,
-// and its softmax would run on one warp.
+// read, so the kernel is built around the copies: six half tiles (128 keys or
+// values, 32 KiB at HD = 128) are in shared memory or on their way. The products
+// use warp-level matrix instructions on 16-row tiles: the 128-row tile of a
+// tcgen05 instruction would be empty but for a few rows, and its softmax would
+// run on one warp.
 //
 // 8 warps share a tile of 128 keys. Warp w takes keys 16w .. 16w + 15 for the
-// scores S = Q K^T (Q from shared memory), makes the weights of those
-// keys and leaves them in shared memory as 16-bit numbers; then it takes the
-// HD / 8 columns w of O = P V for all 128 keys. So K and V are read from shared memory
-// once, O needs no joining across warps, and the only things that the warps
-// share are the weights and a reference maximum per row. The maximum moves when a
-// score passes it by 8 (in powers of two): whether any does is one barrier with
-// an OR, and the exchange of the maxima happens only then.
+// scores S = Q K^T, makes the weights of those keys and leaves them in shared
+// memory as 16-bit numbers; then it takes the HD / 8 columns w of O = P V for all
+// 128 keys. So K and V are read from shared memory once, O needs no joining across
+// warps, and the only things that the warps share are the weights and a reference
+// maximum per row. The maximum moves when a score passes it by 8 (in powers of
+// two): whether any does is one barrier with an OR, and the exchange of the
+// maxima happens only then.
 //
-// A ninth warp walks over the segments (a CTA's part of a unit) and prepares, one
-// tile ahead of the copies, where each key of a tile lies in the cache.
+// A ninth warp walks over the segments (a CTA's part of a unit), prepares where
+// each key of a tile lies and copies the queries and, where a cache block is a
+// whole box of a tensor map (8 rows or more, and a divisor or multiple of 128),
+// keys and values by TMA. Blocks of other sizes are copied row by row with
+// cp.async by four more warps. (The compute warps issuing those copies themselves,
+// between their products, took 2.4 us a tile: 1.6 thousand cycles of the copies'
+// own.)
 #include "tree_attn.cuh"
 
 namespace mcb {
@@ -30,10 +35,15 @@ using namespace tree;
 
 constexpr int WARPS = 8;
 constexpr int COMPUTE = WARPS * 32;
-constexpr int THREADS = COMPUTE + 32;
-constexpr int HALVES = 5;  // half tiles (keys or values) in shared memory
+constexpr int COPIERS = 128;  // threads of the row-by-row copies
+template <bool kTma>
+constexpr int threads() {
+  return COMPUTE + 32 + (kTma ? 0 : COPIERS);
+}
+constexpr int HALVES = 6;  // half tiles (keys or values) in shared memory
 constexpr int TILES = 4;   // ring of prepared tiles
-constexpr int QBUFS = 3;   // query tiles: of the tiles at work, copied and prepared
+constexpr int QBUFS = 2;
+constexpr int CHUNK_BYTES = BK * 128;  // 64 columns of a half tile, 128 bytes a row
 
 struct Tile {
   uint32_t where[BK];  // block << bits | row of each key, kNoRow: nowhere
@@ -49,14 +59,16 @@ struct Smem {
   uint8_t p[16 * MT * BK * 2];  // weights; maxima and sums of the warps in between
   Tile tile[TILES];
   uint64_t full[TILES], empty[TILES];
+  uint64_t kv_full[HALVES], kv_empty[HALVES], q_full[QBUFS], q_empty[QBUFS];
   int64_t start_b;
   int32_t start_w;
   int abort_flag, dirty;
 };
-static_assert(sizeof(Smem<128, 4>) <= 232448, "exceeds the shared memory per block");
+static_assert(sizeof(Smem<128, 2>) <= 232448, "exceeds the shared memory per block");
 
 struct Params : TreeParams {
-  float sign;  // of the scale
+  float sign;         // of the scale
+  int32_t page_rows;  // TMA: rows of a box
 };
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
@@ -88,28 +100,29 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ void tma_load_4d(void *dst, const void *tmap, uint64_t *bar, int32_t x,
+                                            int32_t y, int32_t z, int32_t w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() {
-  asm volatile("cp.async.commit_group;" ::: "memory");
-}
-// Byte offset of 16-byte piece c of a row of BYTES bytes: pieces are permuted
-// within groups of eight by the row, so that eight rows of one piece, or one row
-// of eight, touch all banks.
-template <int BYTES>
+// Byte offset of 16-byte piece c of a row: 64 columns of all ROWS rows after the
+// other, pieces permuted within a row's 128 bytes by the row (TMA's 128-byte
+// swizzle), so that eight rows of one piece, or one row of eight, touch all banks.
+template <int ROWS>
 __device__ __forceinline__ uint32_t piece_at(int row, int c) {
-  return row * BYTES + ((c ^ (row & 7)) << 4);
+  return (c >> 3) * (ROWS * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
 }
 
-template <int HD, int MT, bool kF16>
-__global__ void __launch_bounds__(THREADS) tree_attn_few_kernel(const Params p) {
+template <int HD, int MT, bool kF16, bool kTma>
+__global__ void __launch_bounds__(threads<kTma>())
+    tree_attn_few_kernel(const __grid_constant__ CUtensorMap tk,
+                         const __grid_constant__ CUtensorMap tv, const Params p) {
   constexpr int ROWS = 16 * MT;
-  constexpr int ROW = HD * 2;          // bytes of a key, value or query row
-  constexpr int PIECES = HD / 8;       // 16-byte pieces of a row
-  constexpr int STEP = COMPUTE / PIECES;
-  constexpr int NT = HD / 64;          // 8-column tiles of O per warp
+  constexpr int PIECES = HD / 8;  // 16-byte pieces of a key, value or query row
+  constexpr int NT = HD / 64;     // 8-column tiles of O per warp
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem<HD, MT> &sm = *reinterpret_cast<Smem<HD, MT> *>(smem_raw);
   const TreeAttn &a = p.a;
@@ -120,41 +133,78 @@ __global__ void __launch_bounds__(THREADS) tree_attn_few_kernel(const Params p) 
   if (threadIdx.x == 0) {
     for (int s = 0; s < TILES; ++s) {
       mbar_init(&sm.full[s], 32);
-      mbar_init(&sm.empty[s], COMPUTE);
+      mbar_init(&sm.empty[s], COMPUTE + (kTma ? 0 : COPIERS));
     }
-    sm.abort_flag = sm.dirty = 0;
+    for (int s = 0; s < HALVES; ++s) {
+      mbar_init(&sm.kv_full[s], kTma ? 1 : COPIERS);
+      mbar_init(&sm.kv_empty[s], COMPUTE);
+    }
+    for (int s = 0; s < QBUFS; ++s) {
+      mbar_init(&sm.q_full[s], 32);
+      mbar_init(&sm.q_empty[s], COMPUTE);
+    }
+    // The swizzle needs a 1024-byte aligned base.
+    sm.abort_flag = (smem_u32(smem_raw) & 1023u) != 0;
+    if (sm.abort_flag && p.status) atomicOr(p.status, kErrBadLaunch);
+    sm.dirty = 0;
     fence_mbar_init();
   }
-  const Share share = find_share<ROWS, THREADS>(a, reinterpret_cast<int32_t *>(sm.p), true,
-                                                &sm.start_b, &sm.start_w);
+  if (kTma && warp == WARPS && lane == 0) {
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tv);
+  }
+  const Share share = find_share<ROWS, threads<kTma>()>(
+      a, reinterpret_cast<int32_t *>(sm.p), true, &sm.start_b, &sm.start_w);
 
   if (warp == WARPS) {
-    // ---------------- tiles, one ahead of the copies ----------------
+    // ---------------- tiles, queries and (TMA) keys and values ----------------
     TreeAttnPart part{};
     Walk<ROWS> walk(a, share, part, sm.start_b, sm.start_w);
     Segment sg;
-    uint32_t count = 0;
-    bool ok = true;
-    auto slot = [&]() -> Tile * {
-      const int s = count % TILES;
-      ok = __all_sync(0xffffffffu, mbar_wait(&sm.empty[s], ((count / TILES) & 1) ^ 1, abort_flag,
-                                             p.status, kErrTimeoutEmpty)) != 0;
-      return ok ? &sm.tile[s] : nullptr;
+    uint32_t count = 0, segs = 0;
+    bool ok = !*abort_flag;
+    auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
+      ok = __all_sync(0xffffffffu,
+                      mbar_wait(bar, parity, abort_flag, p.status, kErrTimeoutEmpty)) != 0;
+      return ok;
+    };
+    auto slot_free = [&]() -> bool {
+      return wait(&sm.empty[count % TILES], ((count / TILES) & 1) ^ 1);
     };
     while (ok && walk.next(sg)) {
+      if (!wait(&sm.q_empty[segs % QBUFS], ((segs / QBUFS) & 1) ^ 1)) break;
+      {
+        // Rows past the last one are zero.
+        const int piece = lane % PIECES;
+        const char *q = static_cast<const char *>(a.q) +
+                        (sg.tok0 * a.q_s[0] + sg.head * group * a.q_s[1] + piece * 8) * 2;
+        const uint32_t to = smem_u32(sm.q[segs % QBUFS]);
+#pragma unroll 4
+        for (int r = lane / PIECES; r < ROWS; r += 32 / PIECES) {
+          const bool live = r < sg.nrows;
+          const int row = sg.row0 + (live ? r : 0), tok = fast_div(row, p.group);
+          cp_async16(to + piece_at<ROWS>(r, piece),
+                     q + (tok * a.q_s[0] + (row - tok * group) * a.q_s[1]) * 2, live ? 16 : 0);
+        }
+        cp_async_arrive(&sm.q_full[segs % QBUFS]);
+        ++segs;
+      }
       const int32_t *table = a.table + sg.b * a.table_stride;
-      for (int j = 0; j < sg.ntiles; ++j) {
-        const int key0 = (sg.tile0 + j) * BK;
-        int32_t blk[4];
-        uint32_t col[4];
+      int32_t blk[4];
+      uint32_t col[4];
+      auto look_up = [&](int j) {  // blocks of this lane's keys of tile j
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const int key = key0 + 32 * u + lane;
+          const int key = (sg.tile0 + j) * BK + 32 * u + lane;
           col[u] = fast_div(key, p.block);
-          blk[u] = key < sg.keys ? table[col[u]] : -1;
+          blk[u] = key < sg.keys && j < sg.ntiles ? table[col[u]] : -1;
         }
-        Tile *t = slot();
-        if (!t) break;
+      };
+      look_up(0);
+      for (int j = 0; j < sg.ntiles; ++j) {
+        if (!slot_free()) break;
+        Tile *t = &sm.tile[count % TILES];
+        const int key0 = (sg.tile0 + j) * BK;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int key = key0 + 32 * u + lane;
@@ -169,81 +219,101 @@ __global__ void __launch_bounds__(THREADS) tree_attn_few_kernel(const Params p) 
           t->tile = j;
         }
         mbar_arrive(&sm.full[count % TILES]);
+        look_up(j + 1);
+        if (kTma) {
+          __syncwarp();
+          const int pages = BK / p.page_rows;
+          // Box of this lane: outside the cache (zeros) where there is no block.
+          const uint32_t w = lane < pages ? t->where[lane * p.page_rows] : kNoRow;
+          const int32_t block = w == kNoRow ? static_cast<int32_t>(a.blocks)
+                                            : static_cast<int32_t>(w >> p.row_bits);
+          const int32_t row = w == kNoRow ? 0 : static_cast<int32_t>(w & ((1u << p.row_bits) - 1));
+#pragma unroll
+          for (int value = 0; value < 2; ++value) {
+            const uint32_t half = 2 * count + value, s = half % HALVES;
+            if (!wait(&sm.kv_empty[s], ((half / HALVES) & 1) ^ 1)) break;
+            if (lane == 0) mbar_arrive_expect_tx(&sm.kv_full[s], BK * HD * 2);
+            __syncwarp();
+            if (lane < pages) {
+#pragma unroll
+              for (int c = 0; c < HD / 64; ++c)
+                tma_load_4d(sm.kv[s] + c * CHUNK_BYTES + lane * p.page_rows * 128,
+                            value ? &tv : &tk, &sm.kv_full[s], c * 64, sg.head, row, block);
+            }
+          }
+          if (!ok) break;
+        }
         ++count;
       }
     }
-    // Three ends: the copies look two tiles ahead.
-    for (int k = 0; k < 3 && ok; ++k) {
-      Tile *t = slot();
-      if (!t) break;
-      if (lane == 0) t->seg.kind = kEnd;
+    if (ok && slot_free()) {
+      if (lane == 0) sm.tile[count % TILES].seg.kind = kEnd;
       mbar_arrive(&sm.full[count % TILES]);
-      ++count;
     }
+    cp_async_wait_all();
     if (lane == 0) p.part[blockIdx.x] = part;
     return;
   }
-
-  // ---------------- copies and products ----------------
-  const int tid = threadIdx.x;
-  const int piece = tid % PIECES, r0 = tid / PIECES;
-  const int quad = lane >> 2, ql = lane & 3;
-  auto wait_tile = [&](uint32_t t) -> bool {
-    return mbar_wait(&sm.full[t % TILES], (t / TILES) & 1, abort_flag, p.status, kErrTimeoutFull);
-  };
-  uint32_t qseg = 0;  // segments whose queries were copied
-  // Copies of tile t's keys (value = 0) or values into half 2t + value.
-  auto copy = [&](uint32_t t, int value) {
-    const Tile &d = sm.tile[t % TILES];
-    if (d.seg.kind != kEnd) {
-      const char *base = static_cast<const char *>(value ? a.v : a.k) +
-                         (d.seg.head * (value ? a.v_s[2] : a.k_s[2]) + piece * 8) * 2;
-      const uint32_t blk_step = p.step[value][0], row_step = p.step[value][1];
-      const uint32_t dst = smem_u32(sm.kv[(2 * t + value) % HALVES]);
-#pragma unroll
-      for (int it = 0; it < BK / STEP; ++it) {
-        const int r = r0 + it * STEP;
-        const uint32_t w = d.where[r];
-        const bool none = w == kNoRow;
-        const uint32_t at = (w >> p.row_bits) * blk_step + (w & ((1u << p.row_bits) - 1)) * row_step;
-        cp_async16(dst + piece_at<ROW>(r, piece), base + static_cast<uint64_t>(none ? 0u : at) * 16,
-                   none ? 0 : 16);
-      }
-      if (!value && d.tile == 0) {
-        // The segment's queries; rows past the last one are zero.
-        const Segment &sg = d.seg;
-        const char *q = static_cast<const char *>(a.q) +
-                        (sg.tok0 * a.q_s[0] + sg.head * group * a.q_s[1] + piece * 8) * 2;
-        const uint32_t to = smem_u32(sm.q[qseg % QBUFS]);
-        for (int r = r0; r < ROWS; r += STEP) {
-          const bool live = r < sg.nrows;
-          const int row = sg.row0 + (live ? r : 0), tok = fast_div(row, p.group);
-          cp_async16(to + piece_at<ROW>(r, piece),
-                     q + (tok * a.q_s[0] + (row - tok * group) * a.q_s[1]) * 2, live ? 16 : 0);
+  if (!kTma && warp > WARPS) {
+    // ---------------- row-by-row copies of keys and values ----------------
+    const int tid = threadIdx.x - COMPUTE - 32, piece = tid % PIECES;
+    constexpr int STEP = COPIERS / PIECES;
+    auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
+      return mbar_wait(bar, parity, abort_flag, p.status, kErrTimeoutEmpty);
+    };
+    for (uint32_t t = 0;; ++t) {
+      if (!wait(&sm.full[t % TILES], (t / TILES) & 1)) break;
+      const Tile &d = sm.tile[t % TILES];
+      if (d.seg.kind == kEnd) break;
+      bool ok = true;
+      for (int value = 0; value < 2 && ok; ++value) {
+        const uint32_t half = 2 * t + value, s = half % HALVES;
+        if (!(ok = wait(&sm.kv_empty[s], ((half / HALVES) & 1) ^ 1))) break;
+        const char *base = static_cast<const char *>(value ? a.v : a.k) +
+                           (d.seg.head * (value ? a.v_s[2] : a.k_s[2]) + piece * 8) * 2;
+        const uint32_t blk_step = p.step[value][0], row_step = p.step[value][1];
+        const uint32_t dst = smem_u32(sm.kv[s]);
+#pragma unroll 8
+        for (int r = tid / PIECES; r < BK; r += STEP) {
+          const uint32_t w = d.where[r];
+          const bool none = w == kNoRow;
+          const uint32_t at =
+              (w >> p.row_bits) * blk_step + (w & ((1u << p.row_bits) - 1)) * row_step;
+          cp_async16(dst + piece_at<BK>(r, piece), base + static_cast<uint64_t>(none ? 0u : at) * 16,
+                     none ? 0 : 16);
         }
-        ++qseg;
+        cp_async_arrive(&sm.kv_full[s]);
       }
+      if (!ok) break;
+      mbar_arrive(&sm.empty[t % TILES]);
     }
-    cp_async_commit();
-  };
-  bool ok = true;
-  for (uint32_t t = 0; t < 2; ++t) {
-    ok = ok && wait_tile(t);
-    if (named_bar_or(1, COMPUTE, !ok)) return;
-    copy(t, 0);
-    copy(t, 1);
+    cp_async_wait_all();
+    return;
   }
 
+  // ---------------- products ----------------
+  const int tid = threadIdx.x;
+  const int quad = lane >> 2, ql = lane & 3;
   float o[MT][NT][4], ref[MT][2], l[MT][2];
   uint32_t seg_no = 0;
+  // A warp whose wait runs out says so in the tile's barriers with an OR, so that
+  // all warps leave together.
+  bool ok = true;
+  auto wait = [&](uint64_t *bar, uint32_t parity) {
+    ok = mbar_wait_warp(bar, parity, abort_flag, p.status, kErrTimeoutFull) && ok;
+  };
   for (uint32_t t = 0;; ++t) {
-    // The keys of tile t have landed everywhere, and everyone is done with tile t - 1.
-    cp_async_wait<3>();
-    ok = wait_tile(t + 2);
-    if (named_bar_or(1, COMPUTE, !ok)) return;
+    const uint32_t kh = 2 * t, vh = kh + 1;  // half tiles
+    wait(&sm.full[t % TILES], (t / TILES) & 1);
     const Tile &d = sm.tile[t % TILES];
-    if (d.seg.kind == kEnd) break;
-    copy(t + 2, 0);
+    if (ok && d.seg.kind == kEnd) break;
+    if (ok && d.tile == 0) wait(&sm.q_full[seg_no % QBUFS], (seg_no / QBUFS) & 1);
+    if (ok) wait(&sm.kv_full[kh % HALVES], (kh / HALVES) & 1);
+    if (!ok) {
+      named_bar_or(2, COMPUTE, true);
+      named_bar_or(1, COMPUTE, true);
+      return;
+    }
     if (d.tile == 0) {
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
@@ -262,7 +332,7 @@ __global__ void __launch_bounds__(THREADS) tree_attn_few_kernel(const Params p) 
 #pragma unroll
       for (int n = 0; n < 2; ++n) s[m][n][0] = s[m][n][1] = s[m][n][2] = s[m][n][3] = 0.0f;
     {
-      const uint32_t kb = smem_u32(sm.kv[(2 * t) % HALVES]);
+      const uint32_t kb = smem_u32(sm.kv[kh % HALVES]);
       const uint32_t qb = smem_u32(sm.q[seg_no % QBUFS]);
       // K: matrices (keys 0-7, piece 2k), (0-7, 2k + 1), (8-15, 2k), (8-15, 2k + 1);
       // Q: (rows 0-7, 2k), (8-15, 2k), (0-7, 2k + 1), (8-15, 2k + 1).
@@ -271,16 +341,17 @@ __global__ void __launch_bounds__(THREADS) tree_attn_few_kernel(const Params p) 
 #pragma unroll
       for (int k = 0; k < HD / 16; ++k) {
         uint32_t kf[4];
-        ldmatrix4(kf, kb + piece_at<ROW>(krow, 2 * k + kpc));
+        ldmatrix4(kf, kb + piece_at<BK>(krow, 2 * k + kpc));
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           uint32_t qf[4];
-          ldmatrix4(qf, qb + piece_at<ROW>(16 * m + qrow, 2 * k + qpc));
+          ldmatrix4(qf, qb + piece_at<ROWS>(16 * m + qrow, 2 * k + qpc));
           mma<kF16>(s[m][0], qf, kf[0], kf[1]);
           mma<kF16>(s[m][1], qf, kf[2], kf[3]);
         }
       }
     }
+    mbar_arrive(&sm.kv_empty[kh % HALVES]);
     // ---- masks ----
     const uint32_t good = d.valid[warp >> 1] >> (16 * (warp & 1));
     const bool drafts = pos0 + BK > sg.prefix;  // the tile holds new tokens' keys
@@ -318,6 +389,7 @@ __global__ void __launch_bounds__(THREADS) tree_attn_few_kernel(const Params p) 
         need |= mx > -INFINITY && !((mx - ref[m][h]) * p.c <= 8.0f);
       }
     if (named_bar_or(2, COMPUTE, need)) {
+      if (named_bar_or(1, COMPUTE, false)) return;
       float *most = reinterpret_cast<float *>(sm.p);  // [WARPS][ROWS]
 #pragma unroll
       for (int m = 0; m < MT; ++m)
@@ -361,24 +433,26 @@ __global__ void __launch_bounds__(THREADS) tree_attn_few_kernel(const Params p) 
           const float e0 = ex2(fmaf(s[m][n][2 * h], p.c, -mc));
           const float e1 = ex2(fmaf(s[m][n][2 * h + 1], p.c, -mc));
           l[m][h] += e0 + e1;
-          const uint32_t at =
-              pb + piece_at<BK * 2>(16 * m + quad + 8 * h, 2 * warp + n) + 4 * ql;
+          const uint32_t at = pb + piece_at<ROWS>(16 * m + quad + 8 * h, 2 * warp + n) + 4 * ql;
           asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(pack2<kF16>(e0, e1)) : "memory");
         }
       }
-    // The weights are there and the values have landed; everyone is done with the keys.
-    cp_async_wait<3>();
-    named_bar_sync(3, COMPUTE);
-    copy(t + 2, 1);
-    uint8_t *values = sm.kv[(2 * t + 1) % HALVES];
+    wait(&sm.kv_full[vh % HALVES], (vh / HALVES) & 1);
+    named_bar_sync(3, COMPUTE);  // the weights are there
+    uint8_t *values = sm.kv[vh % HALVES];
     if (drafts) {
       // New tokens' values that are not finite become 0: 0 x inf must not reach
-      // the rows that do not see them. The others add them at the end.
+      // the rows that do not see them. The others add them at the end. Rows past
+      // the last key hold anything and become 0.
       constexpr uint32_t E = kF16 ? 0x7c00u : 0x7f80u;
-      for (int it = 0; it < BK / STEP; ++it) {
-        const int r = r0 + it * STEP;
-        if (pos0 + r < sg.prefix) continue;
-        uint4 *at = reinterpret_cast<uint4 *>(values + piece_at<ROW>(r, piece));
+      for (int i = tid; i < BK * PIECES; i += COMPUTE) {
+        const int r = i / PIECES, pos = pos0 + r;
+        if (pos < sg.prefix) continue;
+        uint4 *at = reinterpret_cast<uint4 *>(values + piece_at<BK>(r, i % PIECES));
+        if (pos >= sg.keys) {
+          *at = make_uint4(0, 0, 0, 0);
+          continue;
+        }
         uint4 w = *at;
         uint32_t *x = reinterpret_cast<uint32_t *>(&w);
         bool bad = false;
@@ -398,6 +472,7 @@ __global__ void __launch_bounds__(THREADS) tree_attn_few_kernel(const Params p) 
           *static_cast<volatile int *>(&sm.dirty) = 1;
         }
       }
+      fence_async_smem();  // before a later TMA copy into the same place
       named_bar_sync(3, COMPUTE);
     }
     // ---- O += P V, this warp's HD / 8 columns ----
@@ -409,9 +484,9 @@ __global__ void __launch_bounds__(THREADS) tree_attn_few_kernel(const Params p) 
       for (int k = 0; k < BK / 16; ++k) {
         uint32_t vf[4];
         if (NT == 2)  // keys 0-7 and 8-15 of the step, pieces 2w and 2w + 1
-          ldmatrix4_trans(vf, vb + piece_at<ROW>(16 * k + (lane & 15), 2 * warp + (lane >> 4)));
+          ldmatrix4_trans(vf, vb + piece_at<BK>(16 * k + (lane & 15), 2 * warp + (lane >> 4)));
         else if (k % 2 == 0)  // one piece, two steps
-          ldmatrix4_trans(vf, vb + piece_at<ROW>(16 * k + lane, warp));
+          ldmatrix4_trans(vf, vb + piece_at<BK>(16 * k + lane, warp));
         if (NT == 1 && k % 2 == 1) {
           vf[0] = held[0];
           vf[1] = held[1];
@@ -422,14 +497,16 @@ __global__ void __launch_bounds__(THREADS) tree_attn_few_kernel(const Params p) 
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           uint32_t pf[4];
-          ldmatrix4(pf, pb + piece_at<BK * 2>(16 * m + prow, 2 * k + ppc));
+          ldmatrix4(pf, pb + piece_at<ROWS>(16 * m + prow, 2 * k + ppc));
           mma<kF16>(o[m][0], pf, vf[0], vf[1]);
           if (NT == 2) mma<kF16>(o[m][NT - 1], pf, vf[2], vf[3]);
         }
       }
     }
+    mbar_arrive(&sm.kv_empty[vh % HALVES]);
     if (d.tile + 1 == sg.ntiles) {
       // ---- the segment's output ----
+      mbar_arrive(&sm.q_empty[seg_no % QBUFS]);
       ++seg_no;
       named_bar_sync(3, COMPUTE);  // the weights are read: sums may take their place
       float *sums = reinterpret_cast<float *>(sm.p);  // [WARPS][ROWS]
@@ -511,32 +588,49 @@ __global__ void __launch_bounds__(THREADS) tree_attn_few_kernel(const Params p) 
     }
     mbar_arrive(&sm.empty[t % TILES]);
   }
-  cp_async_wait<0>();
 }
 
 // Row tiles of 16 that a CTA takes: by the rows that a request has on average.
 int row_tiles(const TreeAttn &a) {
   const int64_t rows = a.tokens * (a.heads / a.kv_heads);
-  return rows <= 16 * a.requests ? 1 : rows <= 32 * a.requests ? 2 : 4;
+  return rows <= 16 * a.requests ? 1 : 2;
 }
 template <int HD, int MT>
 constexpr int per_sm() {  // CTAs that fit into an SM's shared memory (228 KB, 1 KB kept per CTA)
   return 2 * (sizeof(Smem<HD, MT>) + 1024) <= 233472 ? 2 : 1;
 }
 
-template <int HD, int MT, bool kF16>
-cudaError_t run(const TreeAttn &a, void *scratch, uint32_t *status, int sms, cudaStream_t stream,
-                LaunchInfo *info) {
+// Rows of a TMA box, 0 where blocks are no whole boxes.
+int page_rows(const TreeAttn &a) {
+  if (a.block % BK == 0) return BK;
+  return a.block >= 8 && BK % a.block == 0 ? a.block : 0;
+}
+bool cache_map(CUtensorMap *map, const TreeAttn &a, const void *base, const int64_t *st, bool f16,
+               int rows) {
+  const uint64_t dims[4] = {static_cast<uint64_t>(a.dim), static_cast<uint64_t>(a.kv_heads),
+                            static_cast<uint64_t>(a.block), static_cast<uint64_t>(a.blocks)};
+  const uint64_t strides[3] = {static_cast<uint64_t>(st[2]) * 2, static_cast<uint64_t>(st[1]) * 2,
+                               static_cast<uint64_t>(st[0]) * 2};
+  const uint32_t box[4] = {64, 1, static_cast<uint32_t>(rows), 1};
+  return encode_tmap_4d(map,
+                        f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                        base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int HD, int MT, bool kF16, bool kTma>
+cudaError_t run(const TreeAttn &a, const CUtensorMap &tk, const CUtensorMap &tv, void *scratch,
+                uint32_t *status, int sms, cudaStream_t stream, LaunchInfo *info) {
   const int ctas = sms * per_sm<HD, MT>();
   Params p;
   static_cast<TreeParams &>(p) = tree_params(a, scratch, 16 * MT, ctas, status);
   p.sign = a.scale < 0.0f ? -1.0f : 1.0f;
-  auto kernel = tree_attn_few_kernel<HD, MT, kF16>;
+  p.page_rows = page_rows(a);
+  auto kernel = tree_attn_few_kernel<HD, MT, kF16, kTma>;
   constexpr int smem = static_cast<int>(sizeof(Smem<HD, MT>));
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  kernel<<<ctas, THREADS, smem, stream>>>(p);
+  kernel<<<ctas, threads<kTma>(), smem, stream>>>(tk, tv, p);
   tree_attn_join_parts_kernel<HD, 16 * MT, kF16>
       <<<dim3(ctas + 1, 2 * MT), 256, 0, stream>>>(p, ctas);
   info->launches = 2;
@@ -552,11 +646,15 @@ cudaError_t run(const TreeAttn &a, void *scratch, uint32_t *status, int sms, cud
 template <int HD, bool kF16>
 cudaError_t run_rows(const TreeAttn &a, void *scratch, uint32_t *status, int sms,
                      cudaStream_t stream, LaunchInfo *info) {
-  switch (row_tiles(a)) {
-    case 1: return run<HD, 1, kF16>(a, scratch, status, sms, stream, info);
-    case 2: return run<HD, 2, kF16>(a, scratch, status, sms, stream, info);
-    default: return run<HD, 4, kF16>(a, scratch, status, sms, stream, info);
-  }
+  CUtensorMap tk{}, tv{};
+  const int rows = page_rows(a);
+  const bool tma =
+      rows && cache_map(&tk, a, a.k, a.k_s, kF16, rows) && cache_map(&tv, a, a.v, a.v_s, kF16, rows);
+  if (row_tiles(a) == 1)
+    return tma ? run<HD, 1, kF16, true>(a, tk, tv, scratch, status, sms, stream, info)
+               : run<HD, 1, kF16, false>(a, tk, tv, scratch, status, sms, stream, info);
+  return tma ? run<HD, 2, kF16, true>(a, tk, tv, scratch, status, sms, stream, info)
+             : run<HD, 2, kF16, false>(a, tk, tv, scratch, status, sms, stream, info);
 }
 
 }  // namespace
@@ -567,10 +665,10 @@ bool tree_attn_few_ok(const TreeAttn &a, int dtype) {
 }
 
 uint64_t tree_attn_few_scratch(const TreeAttn &a, int sms) {
-  const int mt = row_tiles(a);
-  const int n = a.dim == 128 ? (mt == 1 ? per_sm<128, 1>() : mt == 2 ? per_sm<128, 2>() : per_sm<128, 4>())
-                             : (mt == 1 ? per_sm<64, 1>() : mt == 2 ? per_sm<64, 2>() : per_sm<64, 4>());
-  return tree_scratch(a, 16 * mt, n * sms);
+  const bool one = row_tiles(a) == 1;
+  const int n = a.dim == 128 ? (one ? per_sm<128, 1>() : per_sm<128, 2>())
+                             : (one ? per_sm<64, 1>() : per_sm<64, 2>());
+  return tree_scratch(a, one ? 16 : 32, n * sms);
 }
 
 cudaError_t launch_tree_attn_few(const TreeAttn &a, int dtype, void *scratch, uint32_t *status,

@@ -98,7 +98,7 @@ SHAPES = [  # new, kv, heads, kv_heads, dim, block
 @pytest.mark.parametrize("tree", [True, False])
 def test_sixteen_bits(mcb, shape, dtype, tree):
     new, _, heads, kv_heads = shape[:4]
-    few = sum(new) * (heads // kv_heads) <= 64 * len(new)
+    few = sum(new) * (heads // kv_heads) <= 32 * len(new)
     Case(*shape, dtype, tree).check(
         mcb, "tree_attention_few_rows" if few else "tcgen05_tree_attention")
 
