@@ -71,19 +71,19 @@ bool encode_tmap_3d(CUtensorMap *map, CUtensorMapDataType dtype, const void *bas
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool encode_tmap_4d(CUtensorMap *map, CUtensorMapDataType dtype, const void *base,
+bool encode_tmap_5d(CUtensorMap *map, CUtensorMapDataType dtype, const void *base,
                     const uint64_t *dims, const uint64_t *strides, const uint32_t *box,
                     CUtensorMapSwizzle swizzle) {
   auto fn = encoder();
   if (!fn) return false;
-  cuuint64_t d[4], st[3];
-  cuuint32_t b[4], estr[4] = {1, 1, 1, 1};
-  for (int i = 0; i < 4; ++i) {
+  cuuint64_t d[5], st[4];
+  cuuint32_t b[5], estr[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < 5; ++i) {
     d[i] = dims[i];
     b[i] = box[i];
     if (i > 0) st[i - 1] = dims[i] > 1 ? strides[i - 1] : 16;
   }
-  return fn(map, dtype, 4, const_cast<void *>(base), d, st, b, estr,
+  return fn(map, dtype, 5, const_cast<void *>(base), d, st, b, estr,
             CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }

@@ -341,9 +341,9 @@ bool encode_tmap_3d(CUtensorMap *map, CUtensorMapDataType dtype, const void *bas
                     uint64_t d0, uint64_t d1, uint64_t d2, uint64_t stride1_bytes,
                     uint64_t stride2_bytes, uint32_t box0, uint32_t box1, uint32_t box2,
                     CUtensorMapSwizzle swizzle);
-// dims from the innermost on; byte strides of dims 1..3 (those of a dim of
+// dims from the innermost on; byte strides of dims 1..4 (those of a dim of
 // extent 1 are ignored).
-bool encode_tmap_4d(CUtensorMap *map, CUtensorMapDataType dtype, const void *base,
+bool encode_tmap_5d(CUtensorMap *map, CUtensorMapDataType dtype, const void *base,
                     const uint64_t *dims, const uint64_t *strides, const uint32_t *box,
                     CUtensorMapSwizzle swizzle);
 

@@ -43,7 +43,6 @@ constexpr int threads() {
 constexpr int HALVES = 6;  // half tiles (keys or values) in shared memory
 constexpr int TILES = 4;   // ring of prepared tiles
 constexpr int QBUFS = 2;
-constexpr int CHUNK_BYTES = BK * 128;  // 64 columns of a half tile, 128 bytes a row
 
 struct Tile {
   uint32_t where[BK];  // block << bits | row of each key, kNoRow: nowhere
@@ -68,7 +67,7 @@ static_assert(sizeof(Smem<128, 2>) <= 232448, "exceeds the shared memory per blo
 
 struct Params : TreeParams {
   float sign;         // of the scale
-  int32_t page_rows;  // TMA: rows of a box
+  int32_t page_rows;  // rows of a box (128 without TMA), a power of two
 };
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
@@ -100,20 +99,25 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void tma_load_4d(void *dst, const void *tmap, uint64_t *bar, int32_t x,
-                                            int32_t y, int32_t z, int32_t w) {
+// One box: 64 columns of `page_rows` rows, then the next 64 columns of them.
+__device__ __forceinline__ void tma_load_box(void *dst, const void *tmap, uint64_t *bar,
+                                             int32_t row, int32_t head, int32_t block) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %3, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(0), "r"(row), "r"(head),
+      "r"(block)
       : "memory");
 }
-// Byte offset of 16-byte piece c of a row: 64 columns of all ROWS rows after the
-// other, pieces permuted within a row's 128 bytes by the row (TMA's 128-byte
-// swizzle), so that eight rows of one piece, or one row of eight, touch all banks.
-template <int ROWS>
-__device__ __forceinline__ uint32_t piece_at(int row, int c) {
-  return (c >> 3) * (ROWS * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+// Byte offset of 16-byte piece c of a row of a matrix cut into boxes of `page`
+// rows (a power of two): within a box 64 columns of all rows after the other,
+// within a row's 128 bytes the pieces permuted by the row (TMA's 128-byte swizzle),
+// so that eight rows of one piece, or one row of eight, touch all banks.
+template <int COLS>
+__device__ __forceinline__ uint32_t piece_at(int row, int c, int page) {
+  const uint32_t swz = ((c & 7) ^ (row & 7)) << 4;
+  if (COLS == 64) return row * 128 + swz;
+  return (row + (row & -page) + (c >> 3) * page) * 128 + swz;
 }
 
 template <int HD, int MT, bool kF16, bool kTma>
@@ -183,7 +187,7 @@ __global__ void __launch_bounds__(threads<kTma>())
         for (int r = lane / PIECES; r < ROWS; r += 32 / PIECES) {
           const bool live = r < sg.nrows;
           const int row = sg.row0 + (live ? r : 0), tok = fast_div(row, p.group);
-          cp_async16(to + piece_at<ROWS>(r, piece),
+          cp_async16(to + piece_at<HD>(r, piece, ROWS),
                      q + (tok * a.q_s[0] + (row - tok * group) * a.q_s[1]) * 2, live ? 16 : 0);
         }
         cp_async_arrive(&sm.q_full[segs % QBUFS]);
@@ -234,12 +238,9 @@ __global__ void __launch_bounds__(threads<kTma>())
             if (!wait(&sm.kv_empty[s], ((half / HALVES) & 1) ^ 1)) break;
             if (lane == 0) mbar_arrive_expect_tx(&sm.kv_full[s], BK * HD * 2);
             __syncwarp();
-            if (lane < pages) {
-#pragma unroll
-              for (int c = 0; c < HD / 64; ++c)
-                tma_load_4d(sm.kv[s] + c * CHUNK_BYTES + lane * p.page_rows * 128,
-                            value ? &tv : &tk, &sm.kv_full[s], c * 64, sg.head, row, block);
-            }
+            if (lane < pages)
+              tma_load_box(sm.kv[s] + lane * p.page_rows * (HD * 2), value ? &tv : &tk,
+                           &sm.kv_full[s], row, sg.head, block);
           }
           if (!ok) break;
         }
@@ -279,7 +280,7 @@ __global__ void __launch_bounds__(threads<kTma>())
           const bool none = w == kNoRow;
           const uint32_t at =
               (w >> p.row_bits) * blk_step + (w & ((1u << p.row_bits) - 1)) * row_step;
-          cp_async16(dst + piece_at<BK>(r, piece), base + static_cast<uint64_t>(none ? 0u : at) * 16,
+          cp_async16(dst + piece_at<HD>(r, piece, BK), base + static_cast<uint64_t>(none ? 0u : at) * 16,
                      none ? 0 : 16);
         }
         cp_async_arrive(&sm.kv_full[s]);
@@ -293,7 +294,7 @@ __global__ void __launch_bounds__(threads<kTma>())
 
   // ---------------- products ----------------
   const int tid = threadIdx.x;
-  const int quad = lane >> 2, ql = lane & 3;
+  const int quad = lane >> 2, ql = lane & 3, page = kTma ? p.page_rows : BK;
   float o[MT][NT][4], ref[MT][2], l[MT][2];
   uint32_t seg_no = 0;
   // A warp whose wait runs out says so in the tile's barriers with an OR, so that
@@ -341,11 +342,11 @@ __global__ void __launch_bounds__(threads<kTma>())
 #pragma unroll
       for (int k = 0; k < HD / 16; ++k) {
         uint32_t kf[4];
-        ldmatrix4(kf, kb + piece_at<BK>(krow, 2 * k + kpc));
+        ldmatrix4(kf, kb + piece_at<HD>(krow, 2 * k + kpc, page));
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           uint32_t qf[4];
-          ldmatrix4(qf, qb + piece_at<ROWS>(16 * m + qrow, 2 * k + qpc));
+          ldmatrix4(qf, qb + piece_at<HD>(16 * m + qrow, 2 * k + qpc, ROWS));
           mma<kF16>(s[m][0], qf, kf[0], kf[1]);
           mma<kF16>(s[m][1], qf, kf[2], kf[3]);
         }
@@ -433,7 +434,7 @@ __global__ void __launch_bounds__(threads<kTma>())
           const float e0 = ex2(fmaf(s[m][n][2 * h], p.c, -mc));
           const float e1 = ex2(fmaf(s[m][n][2 * h + 1], p.c, -mc));
           l[m][h] += e0 + e1;
-          const uint32_t at = pb + piece_at<ROWS>(16 * m + quad + 8 * h, 2 * warp + n) + 4 * ql;
+          const uint32_t at = pb + piece_at<BK>(16 * m + quad + 8 * h, 2 * warp + n, ROWS) + 4 * ql;
           asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(pack2<kF16>(e0, e1)) : "memory");
         }
       }
@@ -448,7 +449,7 @@ __global__ void __launch_bounds__(threads<kTma>())
       for (int i = tid; i < BK * PIECES; i += COMPUTE) {
         const int r = i / PIECES, pos = pos0 + r;
         if (pos < sg.prefix) continue;
-        uint4 *at = reinterpret_cast<uint4 *>(values + piece_at<BK>(r, i % PIECES));
+        uint4 *at = reinterpret_cast<uint4 *>(values + piece_at<HD>(r, i % PIECES, page));
         if (pos >= sg.keys) {
           *at = make_uint4(0, 0, 0, 0);
           continue;
@@ -484,9 +485,10 @@ __global__ void __launch_bounds__(threads<kTma>())
       for (int k = 0; k < BK / 16; ++k) {
         uint32_t vf[4];
         if (NT == 2)  // keys 0-7 and 8-15 of the step, pieces 2w and 2w + 1
-          ldmatrix4_trans(vf, vb + piece_at<BK>(16 * k + (lane & 15), 2 * warp + (lane >> 4)));
+          ldmatrix4_trans(vf,
+                          vb + piece_at<HD>(16 * k + (lane & 15), 2 * warp + (lane >> 4), page));
         else if (k % 2 == 0)  // one piece, two steps
-          ldmatrix4_trans(vf, vb + piece_at<BK>(16 * k + lane, warp));
+          ldmatrix4_trans(vf, vb + piece_at<HD>(16 * k + lane, warp, page));
         if (NT == 1 && k % 2 == 1) {
           vf[0] = held[0];
           vf[1] = held[1];
@@ -497,7 +499,7 @@ __global__ void __launch_bounds__(threads<kTma>())
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           uint32_t pf[4];
-          ldmatrix4(pf, pb + piece_at<ROWS>(16 * m + prow, 2 * k + ppc));
+          ldmatrix4(pf, pb + piece_at<BK>(16 * m + prow, 2 * k + ppc, ROWS));
           mma<kF16>(o[m][0], pf, vf[0], vf[1]);
           if (NT == 2) mma<kF16>(o[m][NT - 1], pf, vf[2], vf[3]);
         }
@@ -607,12 +609,13 @@ int page_rows(const TreeAttn &a) {
 }
 bool cache_map(CUtensorMap *map, const TreeAttn &a, const void *base, const int64_t *st, bool f16,
                int rows) {
-  const uint64_t dims[4] = {static_cast<uint64_t>(a.dim), static_cast<uint64_t>(a.kv_heads),
-                            static_cast<uint64_t>(a.block), static_cast<uint64_t>(a.blocks)};
-  const uint64_t strides[3] = {static_cast<uint64_t>(st[2]) * 2, static_cast<uint64_t>(st[1]) * 2,
-                               static_cast<uint64_t>(st[0]) * 2};
-  const uint32_t box[4] = {64, 1, static_cast<uint32_t>(rows), 1};
-  return encode_tmap_4d(map,
+  const uint64_t chunks = a.dim / 64;
+  const uint64_t dims[5] = {64, static_cast<uint64_t>(a.block), chunks,
+                            static_cast<uint64_t>(a.kv_heads), static_cast<uint64_t>(a.blocks)};
+  const uint64_t strides[4] = {static_cast<uint64_t>(st[1]) * 2, 128,
+                               static_cast<uint64_t>(st[2]) * 2, static_cast<uint64_t>(st[0]) * 2};
+  const uint32_t box[5] = {64, static_cast<uint32_t>(rows), static_cast<uint32_t>(chunks), 1, 1};
+  return encode_tmap_5d(map,
                         f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                         base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
@@ -624,7 +627,7 @@ cudaError_t run(const TreeAttn &a, const CUtensorMap &tk, const CUtensorMap &tv,
   Params p;
   static_cast<TreeParams &>(p) = tree_params(a, scratch, 16 * MT, ctas, status);
   p.sign = a.scale < 0.0f ? -1.0f : 1.0f;
-  p.page_rows = page_rows(a);
+  p.page_rows = kTma ? page_rows(a) : BK;
   auto kernel = tree_attn_few_kernel<HD, MT, kF16, kTma>;
   constexpr int smem = static_cast<int>(sizeof(Smem<HD, MT>));
   const cudaError_t e =
