@@ -263,8 +263,8 @@ struct Walk {
   }
 };
 
-// Joins the parts of the units that span CTAs, in their order, one warp a row;
-// the last column of CTAs clears the tokens of no request.
+// Joins the parts of the units that span CTAs, in their order; the last column
+// of CTAs clears the tokens of no request.
 template <int HD, int ROWS, bool kF16>
 __global__ void __launch_bounds__(256) tree_attn_join_parts_kernel(const TreeParams p, int ctas) {
   const TreeAttn &a = p.a;
@@ -291,41 +291,38 @@ __global__ void __launch_bounds__(256) tree_attn_join_parts_kernel(const TreePar
   auto slot = [&](int k) -> int64_t {
     return (static_cast<int64_t>(blockIdx.x) + k) * 2 + (k == 0);
   };
-  constexpr int V = HD / 32;
-  for (int r = blockIdx.y * 8 + warp; r < part.nrows; r += 8 * gridDim.y) {
+  // A part lies by columns of four: column q of row r at q * ROWS + r. A thread
+  // joins one column of one row, neighbours take neighbouring rows.
+  const int rows = (part.nrows + 31) / 32 * 32;
+  for (int w = blockIdx.y * 256 + threadIdx.x; w < rows * (HD / 4); w += 256 * gridDim.y) {
+    const int q = w / rows, r = w - q * rows;
+    if (r >= part.nrows) continue;
     float top = -INFINITY;
-    for (int k = lane; k < part.parts; k += 32) top = fmaxf(top, ml[slot(k) * ROWS + r].x);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+#pragma unroll 4
+    for (int k = 0; k < part.parts; ++k) top = fmaxf(top, ml[slot(k) * ROWS + r].x);
     const float ref = top == -INFINITY ? 0.0f : top;
-    float l = 0.0f, x[V] = {};
+    float l = 0.0f;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
     for (int k = 0; k < part.parts; ++k) {
       const float2 z = ml[slot(k) * ROWS + r];
-      const float w = ex2(z.x - ref);
-      l += z.y * w;
-      const float *in = p.partial + (slot(k) * ROWS + r) * HD + lane * V;
-      float y[V];
-      if (V == 4) {
-        const float4 f = *reinterpret_cast<const float4 *>(in);
-        y[0] = f.x, y[1] = f.y, y[V - 2] = f.z, y[V - 1] = f.w;
-      } else {
-        const float2 f = *reinterpret_cast<const float2 *>(in);
-        y[0] = f.x, y[1] = f.y;
-      }
-#pragma unroll
-      for (int d = 0; d < V; ++d) x[d] = fmaf(y[d], w, x[d]);
+      const float4 y =
+          reinterpret_cast<const float4 *>(p.partial + slot(k) * ROWS * HD)[q * ROWS + r];
+      const float f = ex2(z.x - ref);
+      l = fmaf(z.y, f, l);
+      x.x = fmaf(y.x, f, x.x);
+      x.y = fmaf(y.y, f, x.y);
+      x.z = fmaf(y.z, f, x.z);
+      x.w = fmaf(y.w, f, x.w);
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int row = part.row0 + r, i = row / group;
+    const int row = part.row0 + r, i = fast_div(row, p.group);
     const int64_t tok = static_cast<int64_t>(part.tok0) + i;
     const int head = part.head * group + row - i * group;
-    uint32_t *o = reinterpret_cast<uint32_t *>(static_cast<char *>(a.o) +
-                                               (tok * a.o_s[0] + head * a.o_s[1]) * 2);
-#pragma unroll
-    for (int d = 0; d < V / 2; ++d)
-      o[lane * (V / 2) + d] = pack2<kF16>(x[2 * d] * inv, x[2 * d + 1] * inv);
-    if (lane == 0 && a.lse)
+    *reinterpret_cast<uint2 *>(static_cast<char *>(a.o) +
+                               (tok * a.o_s[0] + head * a.o_s[1] + 4 * q) * 2) =
+        make_uint2(pack2<kF16>(x.x * inv, x.y * inv), pack2<kF16>(x.z * inv, x.w * inv));
+    if (q == 0 && a.lse)
       a.lse[tok * a.lse_s + head] =
           l == 0.0f ? -INFINITY : (ref + log2f(l)) * 0.69314718055994531f;
   }

@@ -577,10 +577,12 @@ __global__ void __launch_bounds__(threads<kTma>())
                   sum == 0.0f ? -INFINITY
                               : ((mc == -INFINITY ? 0.0f : mc) + log2f(sum)) * 0.69314718055994531f;
           } else {
-            float2 *out =
-                reinterpret_cast<float2 *>(p.partial + (part_slot * ROWS + r) * HD + d0);
+            // Columns of four, a row after the other: this pair is half of one.
+            float *out = p.partial + part_slot * ROWS * HD + r * 4 + (ql & 1) * 2;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) out[4 * n] = make_float2(x[n][0], x[n][1]);
+            for (int n = 0; n < NT; ++n)
+              *reinterpret_cast<float2 *>(out + (d0 / 4 + 2 * n) * (ROWS * 4)) =
+                  make_float2(x[n][0], x[n][1]);
             if (warp == 0 && ql == 0)
               reinterpret_cast<float2 *>(p.partial +
                                          static_cast<int64_t>(gridDim.x) * 2 * ROWS *
@@ -635,7 +637,7 @@ cudaError_t run(const TreeAttn &a, const CUtensorMap &tk, const CUtensorMap &tv,
   if (e != cudaSuccess) return e;
   kernel<<<ctas, threads<kTma>(), smem, stream>>>(tk, tv, p);
   tree_attn_join_parts_kernel<HD, 16 * MT, kF16>
-      <<<dim3(ctas + 1, 2 * MT), 256, 0, stream>>>(p, ctas);
+      <<<dim3(ctas + 1, 32 * HD / 4 / 256), 256, 0, stream>>>(p, ctas);
   info->launches = 2;
   info->tile_m = 16 * MT;
   info->tile_n = BK;

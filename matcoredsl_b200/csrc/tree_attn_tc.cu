@@ -12,8 +12,10 @@
 // launch joins them in their order.
 //
 // Two forms of a CTA, both with two softmax warpgroups g = 0, 1 (one thread a
-// row), each with its own scores S_g and output O_g in TMEM and weights P_g in
-// shared memory:
+// row), each with its own scores S_g and output O_g in TMEM; the weights take the
+// scores' place there and are the product's first operand (from shared memory
+// they would cost 64 KiB of writes and 64 KiB of reads a tile on a port that the
+// other operands already fill):
 //   kPair = false  128 rows; warpgroup g takes every second key tile, so that
 //                  the softmax of one tile overlaps the products of the next.
 //                  For few rows the time is the cache's read.
@@ -48,7 +50,7 @@ constexpr int tile_bytes() {
 }
 template <int HD, bool kPair>
 constexpr int stages() {
-  return HD == 128 ? (kPair ? 3 : 4) : (kPair ? 6 : 8);
+  return HD == 128 ? 5 : 8;
 }
 
 struct Params : TreeParams {
@@ -60,7 +62,6 @@ struct Smem {
   static constexpr int ST = stages<HD, kPair>();
   uint8_t q[kPair ? 2 : 1][tile_bytes<HD>()];
   uint8_t kv[ST][tile_bytes<HD>()];
-  uint8_t p[2][128 * BK * 2];
   // Where a tile's keys lie, block << bits | row, kNoRow: nowhere; ordered so that
   // a loader's keys lie together.
   uint32_t info[INFO_RING][BK];
@@ -69,9 +70,10 @@ struct Smem {
   uint64_t seg_full[SEGS], seg_empty[SEGS];
   uint64_t q_full, q_empty;
   uint64_t kv_full[ST], kv_empty[ST];
-  uint64_t s_full[2], s_free[2], p_full[2], p_free[2], o_full[2], o_empty[2];
+  uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
   uint64_t info_ready, join_full, join_read;
   uint64_t drain;
+  float2 joined[kPair ? 1 : 128];  // warpgroup 1's maxima and sums
   int64_t start_b;
   int32_t start_w;
   uint32_t tmem_slot;
@@ -114,9 +116,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
     }
     for (int g = 0; g < 2; ++g) {
       mbar_init(&sm.s_full[g], 1);
-      mbar_init(&sm.s_free[g], 128);
       mbar_init(&sm.p_full[g], 128);
-      mbar_init(&sm.p_free[g], 1);
       mbar_init(&sm.o_full[g], 1);
       mbar_init(&sm.o_empty[g], 128);
     }
@@ -268,10 +268,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
         ok = describe(j) && load(j, false);
       }
       for (int j = 0; j < sg.ntiles && ok; ++j) {
-        if (j + AHEAD < sg.ntiles) {
-          ok = describe(j + AHEAD) && load(j + AHEAD, false);
-        }
-        ok = ok && load(j, true);
+        ok = load(j, true);
+        if (ok && j + AHEAD < sg.ntiles) ok = describe(j + AHEAD) && load(j + AHEAD, false);
       }
       tiles += sg.ntiles;
       if (!ok) break;
@@ -286,8 +284,26 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
       const uint32_t idesc_o = make_idesc(F, F, 0, 1, 128, HD);
       // Bit g: parity of warpgroup g's phase. (Counters indexed by g would live in
       // local memory, whose loads queue behind the loaders' copies.)
-      uint32_t kvc = 0, sc = 0, s_par = 0, p_par = 0, o_par = 0;
+      uint32_t kvc = 0, sc = 0, p_par = 0, o_par = 0;
       bool ok = true;
+      auto stage = [&](uint32_t &addr) -> int {  // the next key or value tile
+        const int s = kvc % ST;
+        if (!mbar_wait(&sm.kv_full[s], (kvc / ST) & 1, abort_flag, p.status, kErrTimeoutFull))
+          return -1;
+        fence_async_smem();
+        tc_fence_after();
+        ++kvc;
+        addr = smem_u32(sm.kv[s]);
+        return s;
+      };
+      auto scores = [&](int g, uint32_t k_addr) {
+        const uint32_t q_addr = smem_u32(sm.q[kPair ? g : 0]);
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+          mma_f16_ss(tmem + S_COL + g * BK, kmajor_desc(q_addr, kk), kmajor_desc(k_addr, kk),
+                     idesc_s, kk ? 1u : 0u);
+        mma_commit(&sm.s_full[g]);
+      };
       for (; ok; ++sc) {
         const int ss = sc % SEGS;
         if (!mbar_wait(&sm.seg_full[ss], (sc / SEGS) & 1, abort_flag, p.status, kErrTimeoutFull))
@@ -298,73 +314,51 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
         const int n = sg.ntiles;
         const int groups = sg.nrows > 128 ? 2 : 1;  // kPair: warpgroups with rows
         if (!mbar_wait(&sm.q_full, sc & 1, abort_flag, p.status, kErrTimeoutFull)) break;
-        fence_async_smem();
-        tc_fence_after();
-        // Scores of tile j: for both row halves, or for the tile's warpgroup.
-        auto scores = [&](int j) -> bool {
-          const int s = kvc % ST;
-          if (!mbar_wait(&sm.kv_full[s], (kvc / ST) & 1, abort_flag, p.status, kErrTimeoutFull))
-            return false;
-          fence_async_smem();
-          ++kvc;
-          const uint32_t k_addr = smem_u32(sm.kv[s]);
-          const int g0 = kPair ? 0 : (j & 1), g1 = kPair ? groups : g0 + 1;
-          for (int g = g0; g < g1; ++g) {
-            if (!mbar_wait(&sm.s_free[g], ((s_par >> g) & 1) ^ 1, abort_flag, p.status,
-                           kErrTimeoutAccum))
-              return false;
-            s_par ^= 1u << g;
-            tc_fence_after();
-            const uint32_t q_addr = smem_u32(sm.q[kPair ? g : 0]);
-#pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk)
-              mma_f16_ss(tmem + S_COL + g * BK, kmajor_desc(q_addr, kk), kmajor_desc(k_addr, kk),
-                         idesc_s, kk ? 1u : 0u);
-            mma_commit(&sm.s_full[g]);
-          }
+        // The first scores; from then on a warpgroup's next scores follow its
+        // product with the values, which has read the weights in their place.
+        for (int j = 0; j < AHEAD && j < n; ++j) {
+          uint32_t k_addr = 0;
+          const int s = stage(k_addr);
+          if (!(ok = s >= 0)) break;
+          scores(kPair ? 0 : j, k_addr);
+          if (kPair && groups == 2) scores(1, k_addr);
           mma_commit(&sm.kv_empty[s]);
-          return true;
-        };
-        auto values = [&](int j) -> bool {
-          const int s = kvc % ST;
-          if (!mbar_wait(&sm.kv_full[s], (kvc / ST) & 1, abort_flag, p.status, kErrTimeoutFull))
-            return false;
-          fence_async_smem();
-          ++kvc;
-          const uint32_t v_addr = smem_u32(sm.kv[s]);
-          const int g0 = kPair ? 0 : (j & 1), g1 = kPair ? groups : g0 + 1;
-          for (int g = g0; g < g1; ++g) {
-            const bool first = kPair ? j == 0 : j < 2;
-            const bool last = kPair ? j + 1 == n : j + 2 >= n;
-            if (first) {
-              if (!mbar_wait(&sm.o_empty[g], ((o_par >> g) & 1) ^ 1, abort_flag, p.status,
-                             kErrTimeoutAccum))
-                return false;
-              o_par ^= 1u << g;
-            }
-            if (!mbar_wait(&sm.p_full[g], (p_par >> g) & 1, abort_flag, p.status, kErrTimeoutAccum))
-              return false;
-            p_par ^= 1u << g;
-            tc_fence_after();
-            const uint32_t p_addr = smem_u32(sm.p[g]);
-#pragma unroll
-            for (int kk = 0; kk < BK / 16; ++kk)
-              mma_f16_ss(tmem + O_COL + g * HD, kmajor_desc(p_addr, kk), mnmajor_desc(v_addr, kk),
-                         idesc_o, (!first || kk) ? 1u : 0u);
-            mma_commit(&sm.p_free[g]);
-            if (last) mma_commit(&sm.o_full[g]);
-          }
-          mma_commit(&sm.kv_empty[s]);
-          return true;
-        };
-        for (int j = 0; j < AHEAD && j < n && ok; ++j) ok = scores(j);
+        }
         if (ok && n <= AHEAD) mma_commit(&sm.q_empty);
         for (int j = 0; j < n && ok; ++j) {
-          if (j + AHEAD < n) {
-            ok = scores(j + AHEAD);
-            if (ok && j + AHEAD + 1 == n) mma_commit(&sm.q_empty);
+          uint32_t v_addr = 0, k_addr = 0;
+          int vs = stage(v_addr), ks = -1;
+          if (!(ok = vs >= 0)) break;
+          const bool first = kPair ? j == 0 : j < 2;
+          const bool last = kPair ? j + 1 == n : j + 2 >= n;
+          const int g0 = kPair ? 0 : (j & 1), g1 = kPair ? groups : g0 + 1;
+          for (int g = g0; g < g1; ++g) {
+            if (first) {
+              if (!(ok = mbar_wait(&sm.o_empty[g], ((o_par >> g) & 1) ^ 1, abort_flag, p.status,
+                                   kErrTimeoutAccum)))
+                break;
+              o_par ^= 1u << g;
+            }
+            if (!(ok = mbar_wait(&sm.p_full[g], (p_par >> g) & 1, abort_flag, p.status,
+                                 kErrTimeoutAccum)))
+              break;
+            p_par ^= 1u << g;
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < BK / 16; ++kk)
+              mma_f16_ts(tmem + O_COL + g * HD, tmem + S_COL + g * BK + kk * 8,
+                         mnmajor_desc(v_addr, kk), idesc_o, (!first || kk) ? 1u : 0u);
+            if (last) mma_commit(&sm.o_full[g]);
+            if (g + 1 == g1) mma_commit(&sm.kv_empty[vs]);
+            if (j + AHEAD < n) {
+              if (g == g0 && !(ok = (ks = stage(k_addr)) >= 0)) break;
+              scores(g, k_addr);
+              if (g + 1 == g1) {
+                mma_commit(&sm.kv_empty[ks]);
+                if (j + AHEAD + 1 == n) mma_commit(&sm.q_empty);
+              }
+            }
           }
-          ok = ok && values(j);
         }
       }
       mma_commit(&sm.drain);
@@ -399,9 +393,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
     const int row = sub * 32 + lane;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(sub * 32) << 16);
     const uint32_t s_col = S_COL + g * BK, o_col = O_COL + g * HD;
-    uint8_t *p_row = sm.p[g] + row * 128;
-    const int rsw = row & 7;
-    uint32_t sc = 0, s_cnt = 0, p_cnt = 0, o_cnt = 0, tiles = 0, joins = 0;
+    uint32_t sc = 0, s_cnt = 0, o_cnt = 0, tiles = 0, joins = 0;
     bool ok = true;
     for (; ok; ++sc) {
       const int ss = sc % SEGS;
@@ -429,12 +421,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
         ++s_cnt;
         tc_fence_after();
         if (!live) {  // no rows: hand the tile on
-          mbar_arrive(&sm.s_free[g]);
-          if (!(ok = mbar_wait_warp(&sm.p_free[g], (p_cnt & 1) ^ 1, abort_flag, p.status,
-                                    kErrTimeoutAccum)))
-            break;
           mbar_arrive(&sm.p_full[g]);
-          ++p_cnt;
           continue;
         }
         uint32_t s[128];
@@ -454,8 +441,6 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
           reg_fence(s2);
           reg_fence(s3);
         }
-        tc_fence_before();
-        mbar_arrive(&sm.s_free[g]);
         const int pos0 = (sg.tile0 + j) * BK;
         const uint4 good = *reinterpret_cast<const uint4 *>(sm.valid[(tiles + j) % VALID_RING]);
         if (pos0 + BK > sg.prefix || (good.x & good.y & good.z & good.w) != 0xffffffffu) {
@@ -486,10 +471,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
         else
           need = (mx - m_ref) * p.c > 8.0f;
         if (__any_sync(0xffffffffu, need)) {
-          if (!(ok = mbar_wait_warp(&sm.p_free[g], (p_cnt - 1) & 1, abort_flag, p.status,
-                                    kErrTimeoutAccum)))
-            break;
-          tc_fence_after();
+          // These scores came after every earlier product with the values.
           const float f = need ? ex2((m_ref - mx) * p.c) : 1.0f;
 #pragma unroll 1
           for (int c0 = 0; c0 < HD; c0 += 16) {
@@ -499,8 +481,6 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
             for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
             tmem_st_32x32b_x16(lane_base + o_col + c0, o);
           }
-          tmem_st_wait();
-          tc_fence_before();
           if (need) {
             l *= f;
             m_ref = mx;
@@ -508,35 +488,31 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
         }
         const float mc = m_ref == -INFINITY ? 0.0f : m_ref * p.c;
         const uint64_t c2 = f2_pack(p.c, p.c), nmc2 = f2_pack(-mc, -mc);
-        uint32_t pk[64];
+        // The weights take the place of the row's scores in TMEM, two a column.
         uint64_t ps[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int k = 0; k < 64; ++k) {
-          float x0, x1;
-          f2_unpack(f2_fma(f2_pack(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), c2,
-                           nmc2),
-                    x0, x1);
-          const float e0 = ex2(x0), e1 = ex2(x1);
-          ps[k & 3] = f2_add(ps[k & 3], f2_pack(e0, e1));
-          pk[k] = pack2<kF16>(e0, e1);
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const int at = 32 * c + 2 * k;
+            float x0, x1;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), c2, nmc2),
+                      x0, x1);
+            const float e0 = ex2(x0), e1 = ex2(x1);
+            ps[k & 3] = f2_add(ps[k & 3], f2_pack(e0, e1));
+            pk[k] = pack2<kF16>(e0, e1);
+          }
+          tmem_st_32x32b_x16(lane_base + s_col + 16 * c, pk);
         }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&sm.p_full[g]);
         {
           float a0, a1;
           f2_unpack(f2_add(f2_add(ps[0], ps[1]), f2_add(ps[2], ps[3])), a0, a1);
           l += a0 + a1;
         }
-        if (!(ok = mbar_wait_warp(&sm.p_free[g], (p_cnt & 1) ^ 1, abort_flag, p.status,
-                                  kErrTimeoutAccum)))
-          break;
-#pragma unroll
-        for (int u = 0; u < 16; ++u) {
-          const int chunk = u >> 3, q = u & 7;
-          *reinterpret_cast<uint4 *>(p_row + chunk * CHUNK_BYTES + ((q ^ rsw) << 4)) =
-              make_uint4(pk[u * 4], pk[u * 4 + 1], pk[u * 4 + 2], pk[u * 4 + 3]);
-        }
-        fence_async_smem();
-        mbar_arrive(&sm.p_full[g]);
-        ++p_cnt;
       }
       if (!ok) break;
       tiles += n;
@@ -552,10 +528,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
         break;
       tc_fence_after();
       if (joined) {
-        // Warpgroup 1 leaves its maximum and sum in its weights' buffer (free
-        // after its last product) and is done; warpgroup 0 reads both outputs,
-        // whose rows lie in the same TMEM lanes.
-        float2 *shared = reinterpret_cast<float2 *>(sm.p[1]);
+        // Warpgroup 1 leaves its maxima and sums and is done; warpgroup 0 reads
+        // both outputs, whose rows lie in the same TMEM lanes.
+        float2 *shared = sm.joined;
         if (g == 1) {
           shared[row] = make_float2(mc, l);
           mbar_arrive(&sm.join_full);
@@ -585,7 +560,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
         const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
         const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (sg.kind == kTail);
         char *orow = static_cast<char *>(a.o) + (tok * a.o_s[0] + head * a.o_s[1]) * 2;
-        float *prow = p.partial + (slot * ROWS + base + row) * HD;
+        // Parts lie by columns of four, so that a warp's rows are stored together.
+        float4 *pcol = reinterpret_cast<float4 *>(p.partial + slot * ROWS * HD) + base + row;
 #pragma unroll 1
         for (int c0 = 0; c0 < HD; c0 += 32) {
           uint32_t o[32];
@@ -632,7 +608,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
             } else {
 #pragma unroll
               for (int q = 0; q < 8; ++q)
-                *reinterpret_cast<float4 *>(prow + c0 + 4 * q) =
+                pcol[(c0 / 4 + q) * ROWS] =
                     make_float4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
             }
           }
