@@ -2204,6 +2204,7 @@ mcb_status rope_impl(const mcb_tensor *q_out, const mcb_tensor *k_out, const mcb
     p.slots = i32(slots);
     p.block = static_cast<int32_t>(k_out->dims[1]);
     p.cache_slots = k_out->dims[0] * k_out->dims[1];
+    p.block_div = mcb::make_div(p.block);
   }
   p.pos_stride = positions->rank == 2 ? positions->strides[0] : 0;
   p.table_stride = cos_sin->strides[0];

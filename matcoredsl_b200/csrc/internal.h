@@ -247,6 +247,26 @@ cudaError_t launch_peer_wait(const uint32_t *flag, uint32_t target, long long li
 // then stores `value` to `flag` (the peer's memory) with release semantics.
 cudaError_t launch_peer_signal(uint32_t *flag, uint32_t value, cudaStream_t stream);
 
+// ---- division by a number known on the host ----------------------------------------------------
+// x / d for x < 2^31: x * ceil(2^(31+s) / d) >> (31+s), 2^s >= d > 2^(s-1). The
+// factor is below 2^32 and the error x * (factor * d - 2^(31+s)) below 2^(31+s).
+struct FastDiv {
+  uint32_t mul;
+  int32_t shift;
+};
+#if defined(__CUDACC__)
+__device__ __forceinline__ uint32_t fast_div(uint32_t x, const FastDiv &d) {
+  return static_cast<uint32_t>((static_cast<uint64_t>(x) * d.mul) >> d.shift);
+}
+#endif
+inline FastDiv make_div(int32_t d) {
+  int s = 0;
+  while ((static_cast<int64_t>(1) << s) < d) ++s;
+  return {static_cast<uint32_t>(((static_cast<uint64_t>(1) << (31 + s)) + d - 1) /
+                                static_cast<uint64_t>(d)),
+          31 + s};
+}
+
 // ---- paged.cu: block tables and slot maps of a paged cache ------------------------------------
 struct PagedGrow {
   int32_t *table, *slots, *positions, *cu, *after, *free_left;
@@ -276,6 +296,7 @@ struct RopeParams {
   int64_t ko_s[3], vo_s[3];  // [token, head], or of a cache [block, row, head]
   int64_t pos_stride, table_stride, table_rows, cache_slots;
   int32_t block, paired, inverse;
+  FastDiv block_div;
   uint8_t axis[kMaxRopePairs];  // position row of each pair
 };
 cudaError_t launch_rope(const RopeParams &p, int dtype, int sms, cudaStream_t stream,

@@ -14,6 +14,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "internal.h"
 
@@ -34,7 +36,7 @@ template <typename T>
 __device__ __forceinline__ T *cache_row(T *base, const RopeParams &p, const int64_t *s,
                                         int32_t slot) {
   if (slot < 0 || slot >= p.cache_slots) return nullptr;
-  const int32_t blk = slot / p.block;
+  const int32_t blk = static_cast<int32_t>(fast_div(slot, p.block_div));
   return base + blk * s[0] + (slot - blk * p.block) * s[1];
 }
 
@@ -98,139 +100,179 @@ __global__ void __launch_bounds__(256) rope_plain_kernel(const RopeParams p) {
   }
 }
 
-// 16 bytes as VE f32 values and back.
+// 16 bytes as VE f32 values, in pairs for the two-element f32 instructions, and back.
 template <typename T>
 struct Vec {
   static constexpr int VE = 16 / sizeof(T);
-  static __device__ __forceinline__ void get(const uint4 &w, float (&f)[VE]) {
-    const T *x = reinterpret_cast<const T *>(&w);
+  static __device__ __forceinline__ void get(const uint4 &v, uint64_t (&f)[VE / 2]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < VE; ++i) f[i] = to_f32(x[i]);
+    for (int i = 0; i < VE / 2; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        f[i] = f2_pack(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+      } else if constexpr (std::is_same_v<T, __half>) {
+        const float2 x = __half22float2(reinterpret_cast<const __half2 &>(w[i]));
+        f[i] = f2_pack(x.x, x.y);
+      } else {
+        f[i] = f2_pack(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+      }
+    }
   }
-  static __device__ __forceinline__ uint4 put(const float (&f)[VE]) {
-    uint4 w;
-    T *x = reinterpret_cast<T *>(&w);
+  static __device__ __forceinline__ uint4 put(const uint64_t (&f)[VE / 2]) {
+    uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < VE; ++i) x[i] = from_f32<T>(f[i]);
-    return w;
+    for (int i = 0; i < VE / 2; ++i) {
+      float lo, hi;
+      f2_unpack(f[i], lo, hi);
+      if constexpr (sizeof(T) == 4) {
+        w[2 * i] = __float_as_uint(lo);
+        w[2 * i + 1] = __float_as_uint(hi);
+      } else if constexpr (std::is_same_v<T, __half>) {
+        w[i] = pack_f16x2(lo, hi);
+      } else {
+        w[i] = pack_bf16x2(lo, hi);
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
 
-// How a CTA of the vector kernel is cut: `tokens` tokens, `slots` head slots
-// of a token, `chunks` threads of a head (VE pairs each).
-struct RopeCut {
-  int tokens, slots, chunks;
-  int table_vec;  // table rows can be read 16 bytes at a time
-};
+constexpr int ROPE_THREADS = 128;
 
-// 16-byte accesses. A thread owns VE pairs: their cosines and sines stay in
-// registers while it walks over the heads of its token, kAhead heads' loads in
-// flight at a time; value rows and elements past the pairs are copied by the
-// same threads.
+// 16-byte accesses. A CTA has threads (chunk of VE pairs, head slot, token): a
+// thread keeps its pairs' cosines and sines in registers while it walks over the
+// heads of its token, kAhead heads' loads in flight at a time; value rows and
+// elements past the pairs are copied by the same threads. The cosines and sines of
+// the CTA's tokens are gathered once into shared memory, after the first loads of
+// q, k and v have been issued. Offsets within a token's rows are 32-bit, there is
+// no division outside the gather of several tokens, and two elements are turned at
+// a time. For 8192 tokens of 32 + 8 + 8 heads of 128 (f16, three axes in turn; HBM
+// floor 31 us): 68 us with every thread gathering its own angles, 55 with a flat
+// thread index that was divided, 51 with 16 slots of 2.5 heads each (what a thread
+// does once per token was more than half of its instructions), 41 as it is.
 template <typename T, bool kPaired, int kAhead>
-__global__ void __launch_bounds__(128) rope_vec_kernel(const RopeParams p, const RopeCut cut) {
+__global__ void __launch_bounds__(ROPE_THREADS) rope_vec_kernel(const RopeParams p) {
   constexpr int VE = Vec<T>::VE;
-  const int per = cut.slots * cut.chunks;
-  const int tok = threadIdx.x / per, r = threadIdx.x - tok * per;
-  const int slot = r / cut.chunks, c = r - slot * cut.chunks;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * cut.tokens + tok;
-  if (tok >= cut.tokens || t >= p.tokens) return;
-  const T *qk[2] = {static_cast<const T *>(p.q) + t * p.q_s[0],
-                    static_cast<const T *>(p.k) + t * p.k_s[0]};
-  T *out[2] = {static_cast<T *>(p.q_out) + t * p.qo_s[0], nullptr};
-  int64_t out_s = p.ko_s[1];
-  T *v_row = nullptr;
-  if (p.slots) {
-    const int32_t at = p.slots[t];
-    out[1] = cache_row(static_cast<T *>(p.k_out), p, p.ko_s, at);
-    out_s = p.ko_s[2];
-    v_row = cache_row(static_cast<T *>(p.v_out), p, p.vo_s, at);
-  } else {
-    out[1] = static_cast<T *>(p.k_out) + t * p.ko_s[0];
-  }
-  const int heads = p.heads + (out[1] ? p.kv_heads : 0);
+  // Tokens of a CTA x pairs <= ROPE_THREADS x VE.
+  __shared__ __align__(16) float cosines[ROPE_THREADS * VE], sines[ROPE_THREADS * VE];
+  const int c = threadIdx.x, slot = threadIdx.y, tok = threadIdx.z;
+  const int chunks = blockDim.x, slots = blockDim.y, tokens = blockDim.z;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * tokens, t = t0 + tok;
+  const bool live = t < p.tokens;
+  const int64_t tl = live ? t : t0;  // dead threads only help with the gather
+  const T *q = static_cast<const T *>(p.q) + tl * p.q_s[0];
+  const T *k = static_cast<const T *>(p.k) + tl * p.k_s[0];
+  const T *v = static_cast<const T *>(p.v) + (p.v ? tl * p.v_s[0] : 0);
+  const int q_s = static_cast<int>(p.q_s[1]), k_s = static_cast<int>(p.k_s[1]);
+  const int v_s = static_cast<int>(p.v_s[1]);
+  const int32_t at = p.slots ? p.slots[tl] : 0;
   // Offsets of the two 16-byte pieces that hold this thread's pairs.
   const int oa = kPaired ? 2 * c * VE : c * VE, ob = kPaired ? oa + VE : p.pairs + c * VE;
-  float cs[VE], sn[VE];
-  // Usually one axis turns all of them: one table row, read 16 bytes at a time.
-  bool one = cut.table_vec;
-#pragma unroll
-  for (int i = 1; i < VE; ++i) one = one && p.axis[c * VE + i] == p.axis[c * VE];
-  const int32_t pos = p.positions[p.axis[c * VE] * p.pos_stride + t];
-  if (one && pos >= 0 && pos < p.table_rows) {
-    const float4 *row = reinterpret_cast<const float4 *>(p.cos_sin + pos * p.table_stride + c * VE);
-    const float4 *sins = reinterpret_cast<const float4 *>(p.cos_sin + pos * p.table_stride +
-                                                          p.pairs + c * VE);
-#pragma unroll
-    for (int i = 0; i < VE / 4; ++i) {
-      const float4 x = row[i], y = sins[i];
-      cs[4 * i] = x.x, cs[4 * i + 1] = x.y, cs[4 * i + 2] = x.z, cs[4 * i + 3] = x.w;
-      sn[4 * i] = y.x, sn[4 * i + 1] = y.y, sn[4 * i + 2] = y.z, sn[4 * i + 3] = y.w;
-    }
-    if (p.inverse) {
-#pragma unroll
-      for (int i = 0; i < VE; ++i) sn[i] = -sn[i];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < VE; ++i) angle(p, t, c * VE + i, cs[i], sn[i]);
-  }
-  for (int h0 = slot; h0 < heads; h0 += kAhead * cut.slots) {
-    uint4 a[kAhead], b[kAhead];
+  const int all_heads = live ? p.heads + p.kv_heads : 0;
+  uint4 a[kAhead], b[kAhead];
+  auto load_heads = [&](int h0) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int h = h0 + u * cut.slots;
-      if (h < heads) {
-        const T *x = h < p.heads ? qk[0] + h * p.q_s[1] : qk[1] + (h - p.heads) * p.k_s[1];
+      const int h = h0 + u * slots;
+      if (h < all_heads) {
+        const T *x = h < p.heads ? q + h * q_s : k + (h - p.heads) * k_s;
         a[u] = *reinterpret_cast<const uint4 *>(x + oa);
         b[u] = *reinterpret_cast<const uint4 *>(x + ob);
       }
     }
+  };
+  load_heads(slot);
+  // Value rows: this thread's first two pieces of its first head ahead.
+  const int v_heads = p.v && live ? p.kv_heads : 0;
+  uint4 v0[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    if (slot < v_heads && (c + u * chunks) * VE < p.dim)
+      v0[u] = *reinterpret_cast<const uint4 *>(v + slot * v_s + (c + u * chunks) * VE);
+  {
+    const int tid = (tok * slots + slot) * chunks + c, threads = chunks * slots * tokens;
+    const int here = static_cast<int>(min(static_cast<int64_t>(tokens), p.tokens - t0));
+    for (int i = tid; i < here * p.pairs; i += threads) {
+      const int gt = tokens == 1 ? 0 : i / p.pairs;
+      angle(p, t0 + gt, i - gt * p.pairs, cosines[i], sines[i]);
+    }
+  }
+  __syncthreads();
+  if (!live) return;
+  T *q_out = static_cast<T *>(p.q_out) + t * p.qo_s[0], *k_out, *v_out = nullptr;
+  const int qo_s = static_cast<int>(p.qo_s[1]);
+  const int ko_s = static_cast<int>(p.slots ? p.ko_s[2] : p.ko_s[1]);
+  if (p.slots) {
+    k_out = cache_row(static_cast<T *>(p.k_out), p, p.ko_s, at);
+    v_out = cache_row(static_cast<T *>(p.v_out), p, p.vo_s, at);
+  } else {
+    k_out = static_cast<T *>(p.k_out) + t * p.ko_s[0];
+  }
+  const int heads = p.heads + (k_out ? p.kv_heads : 0);
+  // Pairs 2i and 2i + 1 of this thread: their cosines, sines and negated sines.
+  uint64_t cs[VE / 2], sn[VE / 2], ns[VE / 2];
+#pragma unroll
+  for (int i = 0; i < VE / 2; ++i) {
+    const float2 x = *reinterpret_cast<const float2 *>(cosines + tok * p.pairs + c * VE + 2 * i);
+    const float2 y = *reinterpret_cast<const float2 *>(sines + tok * p.pairs + c * VE + 2 * i);
+    cs[i] = f2_pack(x.x, x.y);
+    sn[i] = f2_pack(y.x, y.y);
+    ns[i] = f2_pack(-y.x, -y.y);
+  }
+  for (int h0 = slot; h0 < heads; h0 += kAhead * slots) {
+    if (h0 != slot) load_heads(h0);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int h = h0 + u * cut.slots;
+      const int h = h0 + u * slots;
       if (h < heads) {
-        float fa[VE], fb[VE], ga[VE], gb[VE];
+        uint64_t fa[VE / 2], fb[VE / 2], ga[VE / 2], gb[VE / 2];
         Vec<T>::get(a[u], fa);
         Vec<T>::get(b[u], fb);
-        if (kPaired) {
-          // (fa, fb) is 2 VE elements in a row: pair i = elements 2i, 2i + 1.
 #pragma unroll
-          for (int i = 0; i < VE / 2; ++i) {
-            ga[2 * i] = fa[2 * i] * cs[i] - fa[2 * i + 1] * sn[i];
-            ga[2 * i + 1] = fa[2 * i + 1] * cs[i] + fa[2 * i] * sn[i];
-            gb[2 * i] = fb[2 * i] * cs[VE / 2 + i] - fb[2 * i + 1] * sn[VE / 2 + i];
-            gb[2 * i + 1] = fb[2 * i + 1] * cs[VE / 2 + i] + fb[2 * i] * sn[VE / 2 + i];
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < VE; ++i) {
-            ga[i] = fa[i] * cs[i] - fb[i] * sn[i];
-            gb[i] = fb[i] * cs[i] + fa[i] * sn[i];
+        for (int i = 0; i < VE / 2; ++i) {
+          if (kPaired) {
+            // (fa, fb) is 2 VE elements in a row, a pair's two side by side: part them,
+            // turn, and put them back.
+            const uint64_t m = i < VE / 4 ? fa[2 * i] : fb[2 * i - VE / 2];
+            const uint64_t n = i < VE / 4 ? fa[2 * i + 1] : fb[2 * i + 1 - VE / 2];
+            float x0, y0, x1, y1;
+            f2_unpack(m, x0, y0);
+            f2_unpack(n, x1, y1);
+            const uint64_t x = f2_pack(x0, x1), y = f2_pack(y0, y1);
+            const uint64_t gx = f2_fma(x, cs[i], f2_mul(y, ns[i]));
+            const uint64_t gy = f2_fma(y, cs[i], f2_mul(x, sn[i]));
+            f2_unpack(gx, x0, x1);
+            f2_unpack(gy, y0, y1);
+            (i < VE / 4 ? ga[2 * i] : gb[2 * i - VE / 2]) = f2_pack(x0, y0);
+            (i < VE / 4 ? ga[2 * i + 1] : gb[2 * i + 1 - VE / 2]) = f2_pack(x1, y1);
+          } else {
+            ga[i] = f2_fma(fa[i], cs[i], f2_mul(fb[i], ns[i]));
+            gb[i] = f2_fma(fb[i], cs[i], f2_mul(fa[i], sn[i]));
           }
         }
-        T *y = h < p.heads ? out[0] + h * p.qo_s[1] : out[1] + (h - p.heads) * out_s;
+        T *y = h < p.heads ? q_out + h * qo_s : k_out + (h - p.heads) * ko_s;
         *reinterpret_cast<uint4 *>(y + oa) = Vec<T>::put(ga);
         *reinterpret_cast<uint4 *>(y + ob) = Vec<T>::put(gb);
       }
     }
   }
   // Elements past the pairs, then the value rows: plain copies.
-  const int tail = (p.dim - 2 * p.pairs) / VE;
-  for (int i = r; i < heads * tail; i += per) {
-    const int h = i / tail, d = 2 * p.pairs + (i - h * tail) * VE;
-    const T *x = h < p.heads ? qk[0] + h * p.q_s[1] : qk[1] + (h - p.heads) * p.k_s[1];
-    T *y = h < p.heads ? out[0] + h * p.qo_s[1] : out[1] + (h - p.heads) * out_s;
-    *reinterpret_cast<uint4 *>(y + d) = *reinterpret_cast<const uint4 *>(x + d);
-  }
-  if (v_row) {
-    const T *v = static_cast<const T *>(p.v) + t * p.v_s[0];
-    const int pieces = p.dim / VE;
-    for (int i = r; i < p.kv_heads * pieces; i += per) {
-      const int h = i / pieces, d = (i - h * pieces) * VE;
-      *reinterpret_cast<uint4 *>(v_row + h * p.vo_s[2] + d) =
-          *reinterpret_cast<const uint4 *>(v + h * p.v_s[1] + d);
-    }
+  if (2 * p.pairs < p.dim)
+    for (int h = slot; h < heads; h += slots)
+      for (int d = 2 * p.pairs + c * VE; d < p.dim; d += chunks * VE) {
+        const T *x = h < p.heads ? q + h * q_s : k + (h - p.heads) * k_s;
+        T *y = h < p.heads ? q_out + h * qo_s : k_out + (h - p.heads) * ko_s;
+        *reinterpret_cast<uint4 *>(y + d) = *reinterpret_cast<const uint4 *>(x + d);
+      }
+  if (v_out) {
+    const int vo_s = static_cast<int>(p.vo_s[2]);
+    for (int h = slot; h < v_heads; h += slots)
+#pragma unroll 2
+      for (int u = 0; (c + u * chunks) * VE < p.dim; ++u) {
+        const int d = (c + u * chunks) * VE;
+        *reinterpret_cast<uint4 *>(v_out + h * vo_s + d) =
+            h == slot && u < 2 ? v0[u & 1] : *reinterpret_cast<const uint4 *>(v + h * v_s + d);
+      }
   }
 }
 
@@ -243,7 +285,13 @@ bool vector_ok(const RopeParams &p, int ve) {
   int64_t steps = p.dim | p.pairs;
   for (int i = 0; i < 2; ++i) steps |= p.q_s[i] | p.k_s[i] | p.qo_s[i] | (p.v ? p.v_s[i] : 0);
   for (int i = 0; i < (p.slots ? 3 : 2); ++i) steps |= p.ko_s[i] | (p.slots ? p.vo_s[i] : 0);
-  return p.pairs > 0 && bases % 16 == 0 && steps % ve == 0;
+  // 32-bit offsets within a token's rows.
+  int64_t far = 0;
+  for (int64_t x : {(p.heads - 1) * p.q_s[1], (p.heads - 1) * p.qo_s[1],
+                    (p.kv_heads - 1) * p.k_s[1], (p.kv_heads - 1) * p.ko_s[p.slots ? 2 : 1],
+                    p.v ? (p.kv_heads - 1) * p.v_s[1] : 0, p.v ? (p.kv_heads - 1) * p.vo_s[2] : 0})
+    far = x > far ? x : far;
+  return p.pairs > 0 && bases % 16 == 0 && steps % ve == 0 && far + p.dim <= 0x7fffffff;
 }
 
 template <typename T>
@@ -252,20 +300,21 @@ bool run_vec(const RopeParams &p, cudaStream_t stream, LaunchInfo *info) {
   if (!vector_ok(p, VE)) return false;
   const int heads = p.heads + p.kv_heads;
   if (heads == 0) return false;
-  RopeCut cut;
-  cut.chunks = p.pairs / VE;
-  cut.slots = 128 / cut.chunks < heads ? 128 / cut.chunks : heads;
-  cut.tokens = 128 / (cut.chunks * cut.slots);
-  cut.table_vec = reinterpret_cast<uintptr_t>(p.cos_sin) % 16 == 0 && p.table_stride % 4 == 0;
-  const int64_t ctas = (p.tokens + cut.tokens - 1) / cut.tokens;
+  const int chunks = p.pairs / VE;
+  // About five heads a thread: what a thread does once per token (addresses, the
+  // cache's row) is as much as three heads' work.
+  int slots = (heads + 4) / 5;
+  if (slots > ROPE_THREADS / chunks) slots = ROPE_THREADS / chunks;
+  const int tokens = ROPE_THREADS / (chunks * slots) < 64 ? ROPE_THREADS / (chunks * slots) : 64;
+  const int64_t ctas = (p.tokens + tokens - 1) / tokens;
   if (ctas > 0x7fffffff) return false;
-  const unsigned grid = static_cast<unsigned>(ctas);
+  const dim3 block(chunks, slots, tokens);
   if (p.paired)
-    rope_vec_kernel<T, true, 2><<<grid, 128, 0, stream>>>(p, cut);
+    rope_vec_kernel<T, true, 2><<<static_cast<unsigned>(ctas), block, 0, stream>>>(p);
   else
-    rope_vec_kernel<T, false, 2><<<grid, 128, 0, stream>>>(p, cut);
+    rope_vec_kernel<T, false, 2><<<static_cast<unsigned>(ctas), block, 0, stream>>>(p);
   info->launches = 1;
-  info->tile_m = cut.tokens;
+  info->tile_m = tokens;
   info->ctas = static_cast<int>(ctas);
   info->set_route(p.slots ? "rope_append" : "rope");
   return true;

@@ -36,23 +36,6 @@ struct Segment {
 };
 enum : int32_t { kEnd = -1, kWhole = 0, kHead = 1, kTail = 2 };
 
-// x / d for x < 2^31: x * ceil(2^(31+s) / d) >> (31+s), 2^s >= d > 2^(s-1). The
-// factor is below 2^32 and the error x * (factor * d - 2^(31+s)) below 2^(31+s).
-struct FastDiv {
-  uint32_t mul;
-  int32_t shift;
-};
-__device__ __forceinline__ uint32_t fast_div(uint32_t x, const FastDiv &d) {
-  return static_cast<uint32_t>((static_cast<uint64_t>(x) * d.mul) >> d.shift);
-}
-inline FastDiv make_div(int32_t d) {
-  int s = 0;
-  while ((static_cast<int64_t>(1) << s) < d) ++s;
-  return {static_cast<uint32_t>(((static_cast<uint64_t>(1) << (31 + s)) + d - 1) /
-                                static_cast<uint64_t>(d)),
-          31 + s};
-}
-
 struct TreeParams {
   TreeAttn a;
   float c;             // |scale| * log2(e)
