@@ -40,6 +40,7 @@ struct TreeParams {
   TreeAttn a;
   float c;             // |scale| * log2(e)
   FastDiv block, group;
+  int32_t heads_per_kv, most_keys;  // most_keys: what a block table row can hold
   uint32_t step[2][2];  // block and row strides of K and V in 16 bytes
   int32_t row_bits;     // bits of a row within a block
   float *partial;      // [2 * CTAs][ROWS][HD] outputs, then [2 * CTAs][ROWS][2] (max, sum)
@@ -76,37 +77,40 @@ __device__ __forceinline__ void cp_async_wait_all() {
 
 // One request's lengths, clipped to the tensors.
 struct Request {
-  int32_t tok0, n, rows, prefix, keys;  // rows: of the tokens inside [0, T)
+  int32_t tok0, rows, prefix, keys;  // rows: of the tokens inside [0, T)
 };
-__device__ __forceinline__ Request load_request(const TreeAttn &a, int64_t b) {
+__device__ __forceinline__ Request load_request(const TreeParams &p, int64_t b) {
+  const TreeAttn &a = p.a;
   Request r;
   const int64_t c0 = a.cu[b], c1 = a.cu[b + 1], kv = max(0, a.kv_lens[b]);
   const int64_t n = c0 >= 0 && c1 > c0 ? c1 - c0 : 0;
   const int64_t in = max(static_cast<int64_t>(0), min(n, a.tokens - c0));
   r.tok0 = static_cast<int32_t>(c0);
-  r.n = static_cast<int32_t>(n);
-  r.rows = static_cast<int32_t>(in * (a.heads / a.kv_heads));
+  r.rows = static_cast<int32_t>(in) * p.heads_per_kv;
   r.prefix = static_cast<int32_t>(kv - n);
-  r.keys = static_cast<int32_t>(min(kv, a.columns * a.block));
+  r.keys = static_cast<int32_t>(min(kv, static_cast<int64_t>(p.most_keys)));
   return r;
 }
 // Key tiles of row tile `rt`: without a mask the rows see no key past the
 // last one's own.
 template <int ROWS>
-__device__ __forceinline__ int32_t unit_tiles(const TreeAttn &a, const Request &r, int32_t rt) {
-  int64_t end = r.keys;
-  if (!a.mask) {
+__device__ __forceinline__ int32_t unit_tiles(const TreeParams &p, const Request &r, int32_t rt) {
+  int32_t end = r.keys;
+  if (!p.a.mask) {
     const int32_t last = min(r.rows, (rt + 1) * ROWS) - 1;
-    end = min(end, static_cast<int64_t>(r.prefix) + last / (a.heads / a.kv_heads) + 1);
+    const int64_t own = static_cast<int64_t>(r.prefix) + fast_div(last, p.group) + 1;
+    end = static_cast<int32_t>(min(static_cast<int64_t>(end), max(own, static_cast<int64_t>(0))));
   }
-  return end <= BK ? 1 : static_cast<int32_t>((end + BK - 1) / BK);
+  return end <= BK ? 1 : (end + BK - 1) / BK;
 }
+// What a unit costs beside its tiles, in tiles: queries, first scores, output.
+constexpr int32_t kUnitCost = 1;
 template <int ROWS>
-__device__ __forceinline__ int32_t head_tiles(const TreeAttn &a, const Request &r) {
+__device__ __forceinline__ int32_t head_cost(const TreeParams &p, const Request &r) {
   const int32_t rts = (r.rows + ROWS - 1) / ROWS;
-  if (a.mask) return rts * (rts ? unit_tiles<ROWS>(a, r, 0) : 0);
+  if (p.a.mask) return rts ? rts * (unit_tiles<ROWS>(p, r, 0) + kUnitCost) : 0;
   int32_t sum = 0;
-  for (int32_t rt = 0; rt < rts; ++rt) sum += unit_tiles<ROWS>(a, r, rt);
+  for (int32_t rt = 0; rt < rts; ++rt) sum += unit_tiles<ROWS>(p, r, rt) + kUnitCost;
   return sum;
 }
 
@@ -127,22 +131,23 @@ __device__ __forceinline__ uint32_t visible_word(const TreeAttn &a, const uint32
   return s ? (lo >> s) | (word((j >> 5) + 1) << (32 - s)) : lo;
 }
 
-// This CTA's share [w0, w1) of all tiles, found by all THREADS threads of it
+// This CTA's share [w0, w1) of all units' costs, found by all THREADS threads of it
 // (`scan`: THREADS / 32 words of shared memory), and where the requests that hold
-// tile w0 begin. The first `extra` CTAs take share + 1 tiles, the others share.
+// w0 begin. The first `extra` CTAs take share + 1, the others share.
 struct Share {
   int32_t w0, w1, share, extra;
 };
 template <int ROWS, int THREADS>
-__device__ __forceinline__ Share find_share(const TreeAttn &a, int32_t *scan, bool usable,
+__device__ __forceinline__ Share find_share(const TreeParams &p, int32_t *scan, bool usable,
                                             int64_t *start_b, int32_t *start_w) {
+  const TreeAttn &a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t per_thread = (a.requests + THREADS - 1) / THREADS;
   const int64_t b_first = threadIdx.x * per_thread;
   const int64_t b_last = min(a.requests, b_first + per_thread);
   int32_t mine = 0;
   for (int64_t b = b_first; b < b_last; ++b)
-    mine += head_tiles<ROWS>(a, load_request(a, b)) * a.kv_heads;
+    mine += head_cost<ROWS>(p, load_request(p, b)) * a.kv_heads;
   int32_t incl = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -164,7 +169,7 @@ __device__ __forceinline__ Share find_share(const TreeAttn &a, int32_t *scan, bo
   s.extra = works ? total - s.share * ctas : 0;
   s.w0 = cta * s.share + min(cta, s.extra);
   s.w1 = works ? s.w0 + s.share + (cta < s.extra) : s.w0;
-  // The thread whose requests hold tile w0 leaves where they begin.
+  // The thread whose requests hold w0 leaves where they begin.
   if (works && before <= s.w0 && s.w0 < before + mine) {
     *start_b = b_first;
     *start_w = before;
@@ -173,76 +178,82 @@ __device__ __forceinline__ Share find_share(const TreeAttn &a, int32_t *scan, bo
   return s;
 }
 
-// One thread's walk over the segments of a share.
+// One thread's walk over the segments of a share. A unit's cost lies as its tiles,
+// then kUnitCost places that hold none.
 template <int ROWS>
 struct Walk {
-  const TreeAttn &a;
+  const TreeParams &p;
   const Share &sh;
   TreeAttnPart &part;  // the unit that starts in this CTA and ends in a later one
   Request r;
   int64_t b;
-  int32_t w, head = 0, rt = 0, n = 0, tile0 = 0;
+  int32_t w, head = 0, rt = 0, n = 0, at = 0;  // at: place within the unit of n tiles
 
-  __device__ __forceinline__ Walk(const TreeAttn &args, const Share &share, TreeAttnPart &p,
+  __device__ __forceinline__ Walk(const TreeParams &args, const Share &share, TreeAttnPart &first,
                                   int64_t start_b, int32_t start_w)
-      : a(args), sh(share), part(p), b(start_b), w(share.w0) {
+      : p(args), sh(share), part(first), b(start_b), w(share.w0) {
     if (w >= sh.w1) return;
-    int32_t at = start_w;  // first tile of request b
-    r = load_request(a, b);
-    int32_t per = head_tiles<ROWS>(a, r);
-    while (at + per * a.kv_heads <= w) {
-      at += per * a.kv_heads;
-      r = load_request(a, ++b);
-      per = head_tiles<ROWS>(a, r);
+    int32_t from = start_w;  // first place of request b
+    r = load_request(p, b);
+    int32_t per = head_cost<ROWS>(p, r);
+    while (from + per * p.a.kv_heads <= w) {
+      from += per * p.a.kv_heads;
+      r = load_request(p, ++b);
+      per = head_cost<ROWS>(p, r);
     }
-    head = (w - at) / per;
-    tile0 = w - at - head * per;
-    n = unit_tiles<ROWS>(a, r, 0);
-    while (tile0 >= n) {
-      tile0 -= n;
-      n = unit_tiles<ROWS>(a, r, ++rt);
+    head = (w - from) / per;
+    at = w - from - head * per;
+    n = unit_tiles<ROWS>(p, r, 0);
+    while (at >= n + kUnitCost) {
+      at -= n + kUnitCost;
+      n = unit_tiles<ROWS>(p, r, ++rt);
     }
   }
   // False past the last segment.
   __device__ __forceinline__ bool next(Segment &sg) {
-    if (w >= sh.w1) return false;
-    if (n == 0) {  // a new unit
-      if ((rt + 1) * ROWS < r.rows) {
-        ++rt;
-      } else {
-        rt = 0;
-        if (++head == a.kv_heads) {
-          head = 0;
-          do r = load_request(a, ++b);
-          while (r.rows == 0);
+    while (w < sh.w1) {
+      if (at >= n + kUnitCost) {  // a new unit
+        if ((rt + 1) * ROWS < r.rows) {
+          ++rt;
+        } else {
+          rt = 0;
+          if (++head == p.a.kv_heads) {
+            head = 0;
+            do r = load_request(p, ++b);
+            while (r.rows == 0);
+          }
         }
+        n = unit_tiles<ROWS>(p, r, rt);
+        at = 0;
       }
-      n = unit_tiles<ROWS>(a, r, rt);
-      tile0 = 0;
+      const int32_t take = min(n + kUnitCost - at, sh.w1 - w), tile0 = at;
+      const int32_t unit0 = w - at;  // first place of the unit
+      w += take;
+      at += take;
+      const int32_t tiles = min(take, n - tile0);
+      if (tiles <= 0) continue;
+      sg.kind = tile0 > 0 ? kHead : tiles == n ? kWhole : kTail;
+      sg.b = static_cast<int32_t>(b);
+      sg.head = head;
+      sg.row0 = rt * ROWS;
+      sg.nrows = min(r.rows - sg.row0, ROWS);
+      sg.tok0 = r.tok0;
+      sg.prefix = r.prefix;
+      sg.keys = r.keys;
+      sg.tile0 = tile0;
+      sg.ntiles = tiles;
+      if (sg.kind == kTail) {
+        const int32_t last = unit0 + n - 1, big = sh.extra * (sh.share + 1);  // its last tile
+        part.parts = (last < big ? last / (sh.share + 1) : sh.extra + (last - big) / sh.share) -
+                     static_cast<int32_t>(blockIdx.x) + 1;
+        part.tok0 = r.tok0;
+        part.head = head;
+        part.row0 = sg.row0;
+        part.nrows = sg.nrows;
+      }
+      return true;
     }
-    const int32_t take = min(n - tile0, sh.w1 - w);
-    sg.kind = tile0 > 0 ? kHead : take == n ? kWhole : kTail;
-    sg.b = static_cast<int32_t>(b);
-    sg.head = head;
-    sg.row0 = rt * ROWS;
-    sg.nrows = min(r.rows - sg.row0, ROWS);
-    sg.tok0 = r.tok0;
-    sg.prefix = r.prefix;
-    sg.keys = r.keys;
-    sg.tile0 = tile0;
-    sg.ntiles = take;
-    if (sg.kind == kTail) {
-      const int32_t last = w + n - 1, big = sh.extra * (sh.share + 1);  // the unit's last tile
-      part.parts = (last < big ? last / (sh.share + 1) : sh.extra + (last - big) / sh.share) -
-                   static_cast<int32_t>(blockIdx.x) + 1;
-      part.tok0 = r.tok0;
-      part.head = head;
-      part.row0 = sg.row0;
-      part.nrows = sg.nrows;
-    }
-    w += take;
-    n = 0;
-    return true;
+    return false;
   }
 };
 
@@ -250,9 +261,10 @@ struct Walk {
 // of CTAs clears the tokens of no request.
 template <int HD, int ROWS, bool kF16>
 __global__ void __launch_bounds__(256) tree_attn_join_parts_kernel(const TreeParams p, int ctas) {
+  grid_dependency_wait();  // launched while the parts are being made
   const TreeAttn &a = p.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int group = a.heads / a.kv_heads;
+  const int group = p.heads_per_kv;
   if (blockIdx.x == ctas) {
     const int64_t c0 = min(max(static_cast<int64_t>(a.cu[0]), static_cast<int64_t>(0)), a.tokens);
     const int64_t c1 = max(c0, min(static_cast<int64_t>(a.cu[a.requests]), a.tokens));
@@ -280,24 +292,24 @@ __global__ void __launch_bounds__(256) tree_attn_join_parts_kernel(const TreePar
   for (int w = blockIdx.y * 256 + threadIdx.x; w < rows * (HD / 4); w += 256 * gridDim.y) {
     const int q = w / rows, r = w - q * rows;
     if (r >= part.nrows) continue;
-    float top = -INFINITY;
-#pragma unroll 4
-    for (int k = 0; k < part.parts; ++k) top = fmaxf(top, ml[slot(k) * ROWS + r].x);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    float l = 0.0f;
+    // One pass with a running maximum, so that all loads are independent.
+    float top = -INFINITY, l = 0.0f;
     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
+#pragma unroll 8
     for (int k = 0; k < part.parts; ++k) {
       const float2 z = ml[slot(k) * ROWS + r];
       const float4 y =
           reinterpret_cast<const float4 *>(p.partial + slot(k) * ROWS * HD)[q * ROWS + r];
-      const float f = ex2(z.x - ref);
-      l = fmaf(z.y, f, l);
-      x.x = fmaf(y.x, f, x.x);
-      x.y = fmaf(y.y, f, x.y);
-      x.z = fmaf(y.z, f, x.z);
-      x.w = fmaf(y.w, f, x.w);
+      const float m = fmaxf(top, z.x), ref = m == -INFINITY ? 0.0f : m;
+      const float f = ex2(z.x - ref), g = ex2(top - ref);
+      top = m;
+      l = fmaf(z.y, f, l * g);
+      x.x = fmaf(y.x, f, x.x * g);
+      x.y = fmaf(y.y, f, x.y * g);
+      x.z = fmaf(y.z, f, x.z * g);
+      x.w = fmaf(y.w, f, x.w * g);
     }
+    const float ref = top == -INFINITY ? 0.0f : top;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const int row = part.row0 + r, i = fast_div(row, p.group);
     const int64_t tok = static_cast<int64_t>(part.tok0) + i;
@@ -318,7 +330,9 @@ inline TreeParams tree_params(const TreeAttn &a, void *scratch, int rows, int ct
   p.a = a;
   p.c = fabsf(a.scale) * 1.4426950408889634f;
   p.block = make_div(a.block);
-  p.group = make_div(a.heads / a.kv_heads);
+  p.heads_per_kv = a.heads / a.kv_heads;
+  p.group = make_div(p.heads_per_kv);
+  p.most_keys = static_cast<int32_t>(a.columns * a.block);
   for (int i = 0; i < 2; ++i) {
     p.step[0][i] = static_cast<uint32_t>(a.k_s[i] / 8);
     p.step[1][i] = static_cast<uint32_t>(a.v_s[i] / 8);
@@ -329,6 +343,24 @@ inline TreeParams tree_params(const TreeAttn &a, void *scratch, int rows, int ct
                                             static_cast<uint64_t>(ctas) * 2 * rows * (a.dim + 2));
   p.status = status;
   return p;
+}
+// The joining launch, scheduled as the first one's CTAs retire.
+template <int HD, int ROWS, bool kF16>
+cudaError_t launch_join(const TreeParams &p, int ctas, cudaStream_t stream) {
+  const cudaError_t e = cudaGetLastError();  // the first launch's
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  // A thread per four columns of a row, in up to 16 CTAs a unit.
+  constexpr int slices = (ROWS * HD / 4 + 255) / 256;
+  cfg.gridDim = dim3(ctas + 1, slices < 16 ? slices : 16);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, tree_attn_join_parts_kernel<HD, ROWS, kF16>, p, ctas);
 }
 inline uint64_t tree_scratch(const TreeAttn &a, int rows, int ctas) {
   return static_cast<uint64_t>(ctas) *

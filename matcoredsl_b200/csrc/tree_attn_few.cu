@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(threads<kTma>())
   const TreeAttn &a = p.a;
   volatile int *abort_flag = &sm.abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = a.heads / a.kv_heads;
+  const int group = p.heads_per_kv;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < TILES; ++s) {
@@ -157,13 +157,14 @@ __global__ void __launch_bounds__(threads<kTma>())
     tma_prefetch_desc(&tk);
     tma_prefetch_desc(&tv);
   }
+  grid_launch_dependents();
   const Share share = find_share<ROWS, threads<kTma>()>(
-      a, reinterpret_cast<int32_t *>(sm.p), true, &sm.start_b, &sm.start_w);
+      p, reinterpret_cast<int32_t *>(sm.p), true, &sm.start_b, &sm.start_w);
 
   if (warp == WARPS) {
     // ---------------- tiles, queries and (TMA) keys and values ----------------
     TreeAttnPart part{};
-    Walk<ROWS> walk(a, share, part, sm.start_b, sm.start_w);
+    Walk<ROWS> walk(p, share, part, sm.start_b, sm.start_w);
     Segment sg;
     uint32_t count = 0, segs = 0;
     bool ok = !*abort_flag;
@@ -636,8 +637,6 @@ cudaError_t run(const TreeAttn &a, const CUtensorMap &tk, const CUtensorMap &tv,
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   kernel<<<ctas, threads<kTma>(), smem, stream>>>(tk, tv, p);
-  tree_attn_join_parts_kernel<HD, 16 * MT, kF16>
-      <<<dim3(ctas + 1, 32 * HD / 4 / 256), 256, 0, stream>>>(p, ctas);
   info->launches = 2;
   info->tile_m = 16 * MT;
   info->tile_n = BK;
@@ -645,7 +644,7 @@ cudaError_t run(const TreeAttn &a, const CUtensorMap &tk, const CUtensorMap &tv,
   info->stages = HALVES;
   info->ctas = ctas;
   info->set_route("tree_attention_few_rows");
-  return cudaGetLastError();
+  return launch_join<HD, 16 * MT, kF16>(p, ctas, stream);
 }
 
 template <int HD, bool kF16>

@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
   const TreeAttn &a = p.a;
   volatile int *abort_flag = &sm.abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = a.heads / a.kv_heads;
+  const int group = p.heads_per_kv;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < SEGS; ++s) {
@@ -135,12 +135,13 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
     tmem_relinquish();
   }
 
+  grid_launch_dependents();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem_slot;
   const Share share =
-      find_share<ROWS, THREADS>(a, scan, !sm.abort_flag, &sm.start_b, &sm.start_w);
+      find_share<ROWS, THREADS>(p, scan, !sm.abort_flag, &sm.start_b, &sm.start_w);
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
@@ -378,7 +379,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
         ++sc;
         return true;
       };
-      Walk<ROWS> walk(a, share, part, sm.start_b, sm.start_w);
+      Walk<ROWS> walk(p, share, part, sm.start_b, sm.start_w);
       Segment sg;
       while (ok && walk.next(sg)) ok = put(sg);
       p.part[blockIdx.x] = part;
@@ -653,8 +654,7 @@ cudaError_t run(const Params &p, int ctas, cudaStream_t stream) {
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   kernel<<<ctas, THREADS, smem, stream>>>(p);
-  tree_attn_join_parts_kernel<HD, ROWS, kF16><<<dim3(ctas + 1, 8), 256, 0, stream>>>(p, ctas);
-  return cudaGetLastError();
+  return launch_join<HD, ROWS, kF16>(p, ctas, stream);
 }
 
 }  // namespace
