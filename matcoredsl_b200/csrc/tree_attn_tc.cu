@@ -12,17 +12,21 @@
 // launch joins them in their order.
 //
 // Two forms of a CTA, both with two softmax warpgroups g = 0, 1 (one thread a
-// row), each with its own scores S_g and output O_g in TMEM; the weights take the
-// scores' place there and are the product's first operand (from shared memory
-// they would cost 64 KiB of writes and 64 KiB of reads a tile on a port that the
-// other operands already fill):
-//   kPair = false  128 rows; warpgroup g takes every second key tile, so that
-//                  the softmax of one tile overlaps the products of the next.
-//                  For few rows the time is the cache's read.
-//   kPair = true   256 rows, 128 for each warpgroup; each key tile is loaded
-//                  once for both. For wide trees and long runs of new tokens.
+// row), each with its own scores and output O_g in TMEM:
+//   kPair = false  128 rows; a round is two key tiles, one for each warpgroup, so
+//                  that the softmax of one overlaps the products of the other.
+//   kPair = true   256 rows, 128 for each warpgroup; a round is one key tile for
+//                  both. For wide trees and long runs of new tokens.
+// A warpgroup works on half tiles of 64 keys with two score accumulators: the
+// weights take the scores' place and are the first operand of the product with the
+// values, and the scores of the half after the next one follow it there. So one
+// half's scores are always waiting: with whole tiles the softmax waited for
+// product and scores, 5000 cycles for two 128 x 128 tiles of which the tensor core
+// worked 2048. Each warpgroup has its own issuer, because a thread issues a product
+// instruction in about 100 cycles (one issuer for both: 152 us where two take ISSUE us). (From shared memory the weights would cost 64 KiB of writes and 64 KiB
+// of reads a tile on a port that the other operands already fill.)
 // Warps 0-3 load (cp.async: pages may have any size and end inside a tile),
-// 4-7 and 8-11 are the warpgroups, warp 12 issues the products, warp 13 finds
+// 4-7 and 8-11 are the warpgroups, warps 12 and 14 issue their products, warp 13 finds
 // the segments (a CTA's part of a unit) and hands them over a small ring.
 //
 // Keys that a row does not see get the score -inf. Their values must not reach
@@ -37,6 +41,7 @@ using namespace tree;
 
 constexpr int THREADS = 512;
 constexpr int CHUNK_BYTES = 128 * 128;  // 128 rows x 64 16-bit columns, one swizzle span
+constexpr int HALF = BK / 2;  // keys of a score accumulator
 constexpr int LOADERS = 128;
 constexpr int SEGS = 4;         // ring of segments
 constexpr int VALID_RING = 16;  // key tiles whose validity words are kept
@@ -70,9 +75,10 @@ struct Smem {
   uint64_t seg_full[SEGS], seg_empty[SEGS];
   uint64_t q_full, q_empty;
   uint64_t kv_full[ST], kv_empty[ST];
-  uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
+  uint64_t s_full[2][2], p_full[2][2];  // per warpgroup and half tile
+  uint64_t pv_done[2], o_full[2], o_empty[2];
   uint64_t info_ready, join_full, join_read;
-  uint64_t drain;
+  uint64_t drain[2];
   float2 joined[kPair ? 1 : 128];  // warpgroup 1's maxima and sums
   int64_t start_b;
   int32_t start_w;
@@ -94,7 +100,7 @@ template <int HD, bool kPair, bool kF16>
 __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p) {
   constexpr int ST = stages<HD, kPair>();
   constexpr int ROWS = kPair ? 256 : 128;
-  constexpr int AHEAD = kPair ? 1 : 2;  // score tiles issued before the first value tile
+  constexpr int TILES = kPair ? 1 : 2;  // key tiles of a round
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem<HD, kPair> &sm = *reinterpret_cast<Smem<HD, kPair> *>(smem_raw);
   int32_t *scan = reinterpret_cast<int32_t *>(sm.info);  // before the roles start
@@ -106,24 +112,28 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
   if (threadIdx.x == 0) {
     for (int s = 0; s < SEGS; ++s) {
       mbar_init(&sm.seg_full[s], 1);
-      mbar_init(&sm.seg_empty[s], LOADERS + 1 + 256);
+      mbar_init(&sm.seg_empty[s], LOADERS + 2 + 256);
     }
     mbar_init(&sm.q_full, LOADERS);
-    mbar_init(&sm.q_empty, 1);
+    mbar_init(&sm.q_empty, 2);
     for (int s = 0; s < ST; ++s) {
       mbar_init(&sm.kv_full[s], LOADERS);
-      mbar_init(&sm.kv_empty[s], 1);
+      mbar_init(&sm.kv_empty[s], kPair ? 2 : 1);
     }
     for (int g = 0; g < 2; ++g) {
-      mbar_init(&sm.s_full[g], 1);
-      mbar_init(&sm.p_full[g], 128);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&sm.s_full[g][h], 1);
+        mbar_init(&sm.p_full[g][h], 128);
+      }
+      mbar_init(&sm.pv_done[g], 1);
       mbar_init(&sm.o_full[g], 1);
       mbar_init(&sm.o_empty[g], 128);
     }
     mbar_init(&sm.info_ready, LOADERS);
     mbar_init(&sm.join_full, 128);
     mbar_init(&sm.join_read, 128);
-    mbar_init(&sm.drain, 1);
+    mbar_init(&sm.drain[0], 1);
+    mbar_init(&sm.drain[1], 1);
     // The tiles' swizzle needs a 1024-byte aligned base.
     sm.abort_flag = (smem_u32(smem_raw) & 1023u) != 0;
     if (sm.abort_flag && p.status) atomicOr(p.status, kErrBadLaunch);
@@ -265,45 +275,45 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
         }
         return true;
       };
-      for (int j = 0; j < AHEAD && j < sg.ntiles && ok; ++j) {
-        ok = describe(j) && load(j, false);
-      }
-      for (int j = 0; j < sg.ntiles && ok; ++j) {
-        ok = load(j, true);
-        if (ok && j + AHEAD < sg.ntiles) ok = describe(j + AHEAD) && load(j + AHEAD, false);
+      // The order of the products: a round's values, then the next round's keys.
+      for (int j = 0; j < TILES && j < sg.ntiles && ok; ++j) ok = describe(j) && load(j, false);
+      for (int j0 = 0; j0 < sg.ntiles && ok; j0 += TILES) {
+        for (int j = j0; j < j0 + TILES && j < sg.ntiles && ok; ++j) ok = load(j, true);
+        for (int j = j0 + TILES; j < j0 + 2 * TILES && j < sg.ntiles && ok; ++j)
+          ok = describe(j) && load(j, false);
       }
       tiles += sg.ntiles;
       if (!ok) break;
     }
     cp_async_wait_all();
   } else if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 12 && lane == 0) {
-      // ---------------- MMA issuer ----------------
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    if ((warp & 1) == 0 && lane == 0) {
+      // ---------------- MMA issuers: warp 12 for warpgroup 0, warp 14 for 1 ----------------
+      const int g = (warp - 12) >> 1;
       constexpr uint32_t F = kF16 ? 0 : 1;
-      const uint32_t idesc_s = make_idesc(F, F, 0, 0, 128, BK) | p.s_neg;
+      const uint32_t idesc_s = make_idesc(F, F, 0, 0, 128, HALF) | p.s_neg;
       const uint32_t idesc_o = make_idesc(F, F, 0, 1, 128, HD);
-      // Bit g: parity of warpgroup g's phase. (Counters indexed by g would live in
-      // local memory, whose loads queue behind the loaders' copies.)
-      uint32_t kvc = 0, sc = 0, p_par = 0, o_par = 0;
+      const uint32_t s_tmem = tmem + S_COL + g * BK, o_tmem = tmem + O_COL + g * HD;
+      const uint32_t q_addr = smem_u32(sm.q[kPair ? g : 0]);
+      uint32_t kvc = 0, sc = 0, tiles = 0, outs = 0;  // tiles, outs: of this warpgroup
       bool ok = true;
-      auto stage = [&](uint32_t &addr) -> int {  // the next key or value tile
+      // The next key or value tile (kvc counts all tiles, used here or not).
+      auto stage = [&](uint32_t &addr) -> int {
         const int s = kvc % ST;
-        if (!mbar_wait(&sm.kv_full[s], (kvc / ST) & 1, abort_flag, p.status, kErrTimeoutFull))
-          return -1;
+        ok = mbar_wait(&sm.kv_full[s], (kvc / ST) & 1, abort_flag, p.status, kErrTimeoutFull);
         fence_async_smem();
         tc_fence_after();
         ++kvc;
         addr = smem_u32(sm.kv[s]);
         return s;
       };
-      auto scores = [&](int g, uint32_t k_addr) {
-        const uint32_t q_addr = smem_u32(sm.q[kPair ? g : 0]);
+      auto scores = [&](int h, uint32_t k_addr) {  // of half a key tile
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk)
-          mma_f16_ss(tmem + S_COL + g * BK, kmajor_desc(q_addr, kk), kmajor_desc(k_addr, kk),
-                     idesc_s, kk ? 1u : 0u);
-        mma_commit(&sm.s_full[g]);
+          mma_f16_ss(s_tmem + h * HALF, kmajor_desc(q_addr, kk),
+                     kmajor_desc(k_addr + h * (HALF * 128), kk), idesc_s, kk ? 1u : 0u);
+        mma_commit(&sm.s_full[g][h]);
       };
       for (; ok; ++sc) {
         const int ss = sc % SEGS;
@@ -313,57 +323,88 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
         mbar_arrive(&sm.seg_empty[ss]);
         if (sg.kind == kEnd) break;
         const int n = sg.ntiles;
-        const int groups = sg.nrows > 128 ? 2 : 1;  // kPair: warpgroups with rows
         if (!mbar_wait(&sm.q_full, sc & 1, abort_flag, p.status, kErrTimeoutFull)) break;
-        // The first scores; from then on a warpgroup's next scores follow its
-        // product with the values, which has read the weights in their place.
-        for (int j = 0; j < AHEAD && j < n; ++j) {
+        if (kPair ? g * 128 >= sg.nrows : g >= n) {
+          // Nothing to do for this warpgroup: hand everything on.
+          mbar_arrive(&sm.q_empty);
+          if (kPair) {
+            for (int k = 0; k < 2 * n && ok; ++k) {
+              uint32_t addr;
+              const int s = stage(addr);
+              if (ok) mbar_arrive(&sm.kv_empty[s]);
+            }
+          } else {
+            kvc += 2 * n;
+          }
+          continue;
+        }
+        // The first scores. From then on a half's next scores follow the product of
+        // its weights, which lie in their place, with the values: one half's scores
+        // are always ahead. kPair = false: of a round's two tiles the other
+        // warpgroup's is skipped.
+        const int j0 = kPair ? 0 : g;
+        const uint32_t kvc0 = kvc;
+        {
           uint32_t k_addr = 0;
+          kvc += j0;
           const int s = stage(k_addr);
-          if (!(ok = s >= 0)) break;
-          scores(kPair ? 0 : j, k_addr);
-          if (kPair && groups == 2) scores(1, k_addr);
+          if (!ok) break;
+          kvc += min(TILES, n) - 1 - j0;
+          scores(0, k_addr);
+          scores(1, k_addr);
           mma_commit(&sm.kv_empty[s]);
         }
-        if (ok && n <= AHEAD) mma_commit(&sm.q_empty);
-        for (int j = 0; j < n && ok; ++j) {
+        if (j0 + TILES >= n) mma_commit(&sm.q_empty);
+        for (int j = j0; j < n; j += TILES) {
+          const int next = j + TILES, round = j - j0;
           uint32_t v_addr = 0, k_addr = 0;
-          int vs = stage(v_addr), ks = -1;
-          if (!(ok = vs >= 0)) break;
-          const bool first = kPair ? j == 0 : j < 2;
-          const bool last = kPair ? j + 1 == n : j + 2 >= n;
-          const int g0 = kPair ? 0 : (j & 1), g1 = kPair ? groups : g0 + 1;
-          for (int g = g0; g < g1; ++g) {
-            if (first) {
-              if (!(ok = mbar_wait(&sm.o_empty[g], ((o_par >> g) & 1) ^ 1, abort_flag, p.status,
-                                   kErrTimeoutAccum)))
-                break;
-              o_par ^= 1u << g;
-            }
-            if (!(ok = mbar_wait(&sm.p_full[g], (p_par >> g) & 1, abort_flag, p.status,
+          int ks = 0;
+          kvc += j0;
+          const int vs = stage(v_addr);
+          if (!ok) break;
+          kvc += min(TILES, n - round) - 1 - j0;
+          if (j == j0) {
+            if (!(ok = mbar_wait(&sm.o_empty[g], (outs & 1) ^ 1, abort_flag, p.status,
                                  kErrTimeoutAccum)))
               break;
-            p_par ^= 1u << g;
+            ++outs;
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (ok)
+              ok = mbar_wait(&sm.p_full[g][h], tiles & 1, abort_flag, p.status, kErrTimeoutAccum);
+            if (!ok) break;
             tc_fence_after();
 #pragma unroll
-            for (int kk = 0; kk < BK / 16; ++kk)
-              mma_f16_ts(tmem + O_COL + g * HD, tmem + S_COL + g * BK + kk * 8,
-                         mnmajor_desc(v_addr, kk), idesc_o, (!first || kk) ? 1u : 0u);
-            if (last) mma_commit(&sm.o_full[g]);
-            if (g + 1 == g1) mma_commit(&sm.kv_empty[vs]);
-            if (j + AHEAD < n) {
-              if (g == g0 && !(ok = (ks = stage(k_addr)) >= 0)) break;
-              scores(g, k_addr);
-              if (g + 1 == g1) {
+            for (int kk = 0; kk < HALF / 16; ++kk)
+              mma_f16_ts(o_tmem, s_tmem + h * HALF + kk * 8,
+                         mnmajor_desc(v_addr, h * (HALF / 16) + kk), idesc_o,
+                         (round || h || kk) ? 1u : 0u);
+            mma_commit(&sm.pv_done[g]);
+            if (h == 1) {
+              if (next >= n) mma_commit(&sm.o_full[g]);
+              mma_commit(&sm.kv_empty[vs]);
+            }
+            if (next < n) {
+              if (h == 0) {
+                kvc += j0;
+                ks = stage(k_addr);
+                if (!ok) break;
+                kvc += min(TILES, n - round - TILES) - 1 - j0;
+              }
+              scores(h, k_addr);
+              if (h == 1) {
                 mma_commit(&sm.kv_empty[ks]);
-                if (j + AHEAD + 1 == n) mma_commit(&sm.q_empty);
+                if (next + TILES >= n) mma_commit(&sm.q_empty);
               }
             }
           }
+          ++tiles;
         }
+        kvc = kvc0 + 2 * n;
       }
-      mma_commit(&sm.drain);
-      if (!mbar_wait(&sm.drain, 0, nullptr, p.status, kErrTimeoutDrain)) *abort_flag = 1;
+      mma_commit(&sm.drain[g]);
+      if (!mbar_wait(&sm.drain[g], 0, nullptr, p.status, kErrTimeoutDrain)) *abort_flag = 1;
     } else if (warp == 13 && lane == 0) {
       // ---------------- scheduler ----------------
       uint32_t sc = 0;
@@ -388,13 +429,13 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
       if (ok) put(end);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     // ---------------- softmax and output ----------------
     const int g = (warp - 4) >> 2, sub = warp & 3;
     const int row = sub * 32 + lane;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(sub * 32) << 16);
     const uint32_t s_col = S_COL + g * BK, o_col = O_COL + g * HD;
-    uint32_t sc = 0, s_cnt = 0, o_cnt = 0, tiles = 0, joins = 0;
+    uint32_t sc = 0, steps = 0, o_cnt = 0, tiles = 0, joins = 0;
     bool ok = true;
     for (; ok; ++sc) {
       const int ss = sc % SEGS;
@@ -415,40 +456,36 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
       const uint32_t *mask_row =
           a.mask ? a.mask + (static_cast<int64_t>(sg.tok0) + i) * a.mask_stride : nullptr;
       float m_ref = -INFINITY, l = 0.0f;
-      for (int j = j0; j < n && busy; j += step) {
-        if (!(ok = mbar_wait_warp(&sm.s_full[g], s_cnt & 1, abort_flag, p.status,
+      for (int j2 = 2 * j0; j2 < 2 * n && busy; j2 += (j2 & 1) ? 2 * step - 1 : 1) {
+        const int j = j2 >> 1, h = j2 & 1;  // tile, half
+        if (!(ok = mbar_wait_warp(&sm.s_full[g][h], (steps >> 1) & 1, abort_flag, p.status,
                                   kErrTimeoutAccum)))
           break;
-        ++s_cnt;
+        ++steps;
         tc_fence_after();
-        if (!live) {  // no rows: hand the tile on
-          mbar_arrive(&sm.p_full[g]);
+        if (!live) {  // no rows: hand the half on
+          mbar_arrive(&sm.p_full[g][h]);
           continue;
         }
-        uint32_t s[128];
+        const uint32_t at = lane_base + s_col + h * HALF;
+        uint32_t s[HALF];
         {
           uint32_t (&s0)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[0]);
           uint32_t (&s1)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[32]);
-          uint32_t (&s2)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[64]);
-          uint32_t (&s3)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[96]);
-          const uint32_t at = lane_base + s_col;
           tmem_ld_32x32b_x32(at, s0);
           tmem_ld_32x32b_x32(at + 32, s1);
-          tmem_ld_32x32b_x32(at + 64, s2);
-          tmem_ld_32x32b_x32(at + 96, s3);
           tmem_ld_wait();
           reg_fence(s0);
           reg_fence(s1);
-          reg_fence(s2);
-          reg_fence(s3);
         }
-        const int pos0 = (sg.tile0 + j) * BK;
-        const uint4 good = *reinterpret_cast<const uint4 *>(sm.valid[(tiles + j) % VALID_RING]);
-        if (pos0 + BK > sg.prefix || (good.x & good.y & good.z & good.w) != 0xffffffffu) {
-          const uint32_t gw[4] = {good.x, good.y, good.z, good.w};
+        const int pos0 = (sg.tile0 + j) * BK + h * HALF;
+        const uint2 good =
+            *reinterpret_cast<const uint2 *>(sm.valid[(tiles + j) % VALID_RING] + 2 * h);
+        if (pos0 + HALF > sg.prefix || (good.x & good.y) != 0xffffffffu) {
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t see = gw[w] & visible_word(a, mask_row, pos0 + 32 * w, sg.prefix, i);
+          for (int w = 0; w < 2; ++w) {
+            const uint32_t see = (w ? good.y : good.x) &
+                                 visible_word(a, mask_row, pos0 + 32 * w, sg.prefix, i);
 #pragma unroll
             for (int k = 0; k < 32; ++k)
               if (!((see >> k) & 1u)) s[32 * w + k] = 0xff800000u;
@@ -456,13 +493,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
         }
         float m4[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) m4[k] = __uint_as_float(s[k]);
+        for (int q = 0; q < 4; ++q) {
+          m4[q] = fmaxf(__uint_as_float(s[q]), __uint_as_float(s[q + 4]));
 #pragma unroll
-        for (int k = 4; k < 128; k += 8)
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            m4[q] = fmax3(m4[q], __uint_as_float(s[(k + 2 * q) & 127]),
-                          __uint_as_float(s[(k + 2 * q + 1) & 127]));
+          for (int k = 8; k < HALF; k += 8)
+            m4[q] = fmax3(m4[q], __uint_as_float(s[k + q]), __uint_as_float(s[k + q + 4]));
+        }
         const float mx = fmax3(m4[0], m4[1], fmaxf(m4[2], m4[3]));
         // The reference maximum moves only when a weight would pass 2^8. While
         // it is -inf, O and l are zero.
@@ -472,7 +508,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
         else
           need = (mx - m_ref) * p.c > 8.0f;
         if (__any_sync(0xffffffffu, need)) {
-          // These scores came after every earlier product with the values.
+          // O is at rest once the previous half's product is done: this half's
+          // waits for these weights.
+          if (!(ok = mbar_wait_warp(&sm.pv_done[g], (steps - 2) & 1, abort_flag, p.status,
+                                    kErrTimeoutAccum)))
+            break;
+          tc_fence_after();
           const float f = need ? ex2((m_ref - mx) * p.c) : 1.0f;
 #pragma unroll 1
           for (int c0 = 0; c0 < HD; c0 += 16) {
@@ -492,23 +533,23 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
         // The weights take the place of the row's scores in TMEM, two a column.
         uint64_t ps[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           uint32_t pk[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
-            const int at = 32 * c + 2 * k;
+            const int e = 32 * c + 2 * k;
             float x0, x1;
-            f2_unpack(f2_fma(f2_pack(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), c2, nmc2),
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, nmc2),
                       x0, x1);
             const float e0 = ex2(x0), e1 = ex2(x1);
             ps[k & 3] = f2_add(ps[k & 3], f2_pack(e0, e1));
             pk[k] = pack2<kF16>(e0, e1);
           }
-          tmem_st_32x32b_x16(lane_base + s_col + 16 * c, pk);
+          tmem_st_32x32b_x16(at + 16 * c, pk);
         }
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(&sm.p_full[g]);
+        mbar_arrive(&sm.p_full[g][h]);
         {
           float a0, a1;
           f2_unpack(f2_add(f2_add(ps[0], ps[1]), f2_add(ps[2], ps[3])), a0, a1);
