@@ -103,14 +103,19 @@ __device__ __forceinline__ int32_t unit_tiles(const TreeParams &p, const Request
   }
   return end <= BK ? 1 : (end + BK - 1) / BK;
 }
-// What a unit costs beside its tiles, in tiles: queries, first scores, output.
-constexpr int32_t kUnitCost = 1;
+// What a unit costs beside its tiles, in tiles: queries, first scores, output. 16 or
+// 32 rows: 1 (2 and 3 made decoding of 64 requests with up to 1000 keys 3 and 10%
+// slower); 128 or 256 rows: 3 (1 made 24 wide trees 15% slower).
+template <int ROWS>
+constexpr int32_t unit_cost() {
+  return ROWS <= 32 ? 1 : 3;
+}
 template <int ROWS>
 __device__ __forceinline__ int32_t head_cost(const TreeParams &p, const Request &r) {
   const int32_t rts = (r.rows + ROWS - 1) / ROWS;
-  if (p.a.mask) return rts ? rts * (unit_tiles<ROWS>(p, r, 0) + kUnitCost) : 0;
+  if (p.a.mask) return rts ? rts * (unit_tiles<ROWS>(p, r, 0) + unit_cost<ROWS>()) : 0;
   int32_t sum = 0;
-  for (int32_t rt = 0; rt < rts; ++rt) sum += unit_tiles<ROWS>(p, r, rt) + kUnitCost;
+  for (int32_t rt = 0; rt < rts; ++rt) sum += unit_tiles<ROWS>(p, r, rt) + unit_cost<ROWS>();
   return sum;
 }
 
@@ -179,7 +184,7 @@ __device__ __forceinline__ Share find_share(const TreeParams &p, int32_t *scan, 
 }
 
 // One thread's walk over the segments of a share. A unit's cost lies as its tiles,
-// then kUnitCost places that hold none.
+// then unit_cost() places that hold none.
 template <int ROWS>
 struct Walk {
   const TreeParams &p;
@@ -204,15 +209,15 @@ struct Walk {
     head = (w - from) / per;
     at = w - from - head * per;
     n = unit_tiles<ROWS>(p, r, 0);
-    while (at >= n + kUnitCost) {
-      at -= n + kUnitCost;
+    while (at >= n + unit_cost<ROWS>()) {
+      at -= n + unit_cost<ROWS>();
       n = unit_tiles<ROWS>(p, r, ++rt);
     }
   }
   // False past the last segment.
   __device__ __forceinline__ bool next(Segment &sg) {
     while (w < sh.w1) {
-      if (at >= n + kUnitCost) {  // a new unit
+      if (at >= n + unit_cost<ROWS>()) {  // a new unit
         if ((rt + 1) * ROWS < r.rows) {
           ++rt;
         } else {
@@ -226,7 +231,7 @@ struct Walk {
         n = unit_tiles<ROWS>(p, r, rt);
         at = 0;
       }
-      const int32_t take = min(n + kUnitCost - at, sh.w1 - w), tile0 = at;
+      const int32_t take = min(n + unit_cost<ROWS>() - at, sh.w1 - w), tile0 = at;
       const int32_t unit0 = w - at;  // first place of the unit
       w += take;
       at += take;

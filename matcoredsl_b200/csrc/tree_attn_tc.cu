@@ -23,7 +23,7 @@
 // half's scores are always waiting: with whole tiles the softmax waited for
 // product and scores, 5000 cycles for two 128 x 128 tiles of which the tensor core
 // worked 2048. Each warpgroup has its own issuer, because a thread issues a product
-// instruction in about 100 cycles (one issuer for both: 152 us where two take ISSUE us). (From shared memory the weights would cost 64 KiB of writes and 64 KiB
+// instruction in about 100 cycles (24 wide trees: 152 us with one issuer for both, 118 with two). (From shared memory the weights would cost 64 KiB of writes and 64 KiB
 // of reads a tile on a port that the other operands already fill.)
 // Warps 0-3 load (cp.async: pages may have any size and end inside a tile),
 // 4-7 and 8-11 are the warpgroups, warps 12 and 14 issue their products, warp 13 finds
