@@ -22,9 +22,13 @@
 // values, and the scores of the half after the next one follow it there. So one
 // half's scores are always waiting: with whole tiles the softmax waited for
 // product and scores, 5000 cycles for two 128 x 128 tiles of which the tensor core
-// worked 2048. Each warpgroup has its own issuer, because a thread issues a product
-// instruction in about 100 cycles (24 wide trees: 152 us with one issuer for both, 118 with two). (From shared memory the weights would cost 64 KiB of writes and 64 KiB
-// of reads a tile on a port that the other operands already fill.)
+// worked 2048. Each warpgroup has its own issuer, because one thread takes about 100
+// cycles for a product instruction (24 wide trees: 152 us with one issuer for both,
+// 118 with two). From shared memory the weights would cost 64 KiB of writes and
+// 64 KiB of reads a tile on a port that the other operands already fill. Five stages
+// of keys and values, and outputs stored row by row: a fifth stage given up for
+// storing them through shared memory made long contexts 7% slower and short ones no
+// faster.
 // Warps 0-3 load (cp.async: pages may have any size and end inside a tile),
 // 4-7 and 8-11 are the warpgroups, warps 12 and 14 issue their products, warp 13 finds
 // the segments (a CTA's part of a unit) and hands them over a small ring.
