@@ -2,7 +2,8 @@
  * mcb.h -- C ABI of the B200 (sm_100a) implementation of MatcoreDSL's
  * data-parallel hot path: strict f32 GEMM and fused GEMM pair, bf16 GEMM with
  * a fused epilogue (Family A), matmul-softmax-matmul (Family C), the FP8
- * block-scaled GEMM, and the attention-residual block region.
+ * block-scaled GEMM, and the attention-residual block region; and of the
+ * operators of a serving step over a paged key/value cache.
  *
  * Every entry point is extern "C", noexcept, takes plain pointers and sizes,
  * and reports failure only through its return code. Each declaration names
@@ -681,10 +682,15 @@ MCB_API mcb_status mcb_rope_append_v1(const mcb_tensor *q_out, const mcb_tensor 
  * columns and of table entries outside the cache are not seen. What is not
  * seen has no influence, NaN and infinities included.
  * q, o and the caches share one type (bf16, f16, f32), dim <= 256. bf16 and
- * f16 with dim 64 or 128 and 16-byte aligned bases and strides run on
- * tcgen05 (the weights rounded to the 16-bit type for the second product,
- * statistics and sums in f32), all else on CUDA cores in f32. Scratch for
- * partial results of long contexts: see Scratch above. */
+ * f16 with dim 64 or 128, 16-byte aligned bases and strides and a scale other
+ * than 0 run on tensor cores (the weights rounded to the 16-bit type for the
+ * second product, statistics and sums in f32): requests of up to 32 rows (new
+ * tokens x heads per key head) on average on 16-row tiles
+ * ("tree_attention_few_rows"), more on tcgen05 ("tcgen05_tree_attention"). All
+ * else runs on CUDA cores in f32 ("simt_tree_attention"). Any block size is
+ * taken; powers of two from 8 to 128 and multiples of 128 are copied by TMA on
+ * the first route. Scratch for partial results of contexts that several CTAs
+ * share: see Scratch above (up to 40 MB on the tensor-core routes). */
 MCB_API mcb_status mcb_tree_attention_v1(const mcb_tensor *o, const mcb_tensor *lse,
                                          const mcb_tensor *q, const mcb_tensor *k_cache,
                                          const mcb_tensor *v_cache,
@@ -699,6 +705,7 @@ MCB_API mcb_status mcb_tree_attention_v1(const mcb_tensor *o, const mcb_tensor *
  * token_ids[cu_tokens[r] .. cu_tokens[r+1]), its first prompt_lens[r] the
  * prompt, the rest generated. In f32, in this order, rounded once:
  *   v in the history:   x = x > 0 ? x / repetition[r] : x * repetition[r]
+ *                       (the division as a product with 1 / repetition[r])
  *   v generated n > 0 times: x = x - frequency[r] * n - presence[r]
  *   v in the row's list bias_ids[bias_cu[r] .. bias_cu[r+1]):
  *                       x = x + its bias_values entry (its last, if several)

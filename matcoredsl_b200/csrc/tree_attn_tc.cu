@@ -708,6 +708,7 @@ bool tree_attn_tc_ok(const TreeAttn &a, int dtype) {
   if (dtype != MCB_DTYPE_BF16 && dtype != MCB_DTYPE_F16) return false;
   if (a.dim != 64 && a.dim != 128) return false;
   if (a.scale == 0.0f) return false;  // a masked score times 0 would be NaN
+  if (a.blocks == 0) return false;    // no cache row to point copies of nothing at
   const uintptr_t bases = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) |
                           reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.o);
   int64_t steps = a.q_s[0] | a.q_s[1] | a.o_s[0] | a.o_s[1];

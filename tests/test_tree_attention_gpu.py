@@ -90,7 +90,9 @@ SHAPES = [  # new, kv, heads, kv_heads, dim, block
     ([2] * 70, [i * 5 + 2 for i in range(70)], 4, 4, 64, 64),
     ([130], [400], 4, 2, 128, 128),
     ([7], [3000], 16, 1, 128, 48),
-    ([9, 1], [20, 2500], 40, 8, 128, 1)]
+    ([9, 1], [20, 2500], 40, 8, 128, 1),
+    ([3], [1000], 8, 2, 64, 256),
+    ([33], [700], 8, 2, 128, 256)]
 
 
 @pytest.mark.parametrize("shape", SHAPES)
@@ -198,6 +200,17 @@ def test_tables(mcb, dtype):
     c.cu = np.array([0, 2, 4])  # the fifth token belongs to nobody
     c.check(mcb)
     c.kv[1] = -5
+    c.check(mcb)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_no_request_and_no_block(mcb, dtype):
+    """Tokens of no request at all; a cache without blocks: zeros, and -inf."""
+    c = Case([3], [30], 8, 2, 128, 16, dtype)
+    c.cu, c.kv, c.table = np.array([0]), np.array([], np.int64), c.table[:0]
+    c.check(mcb)
+    c = Case([3], [30], 8, 2, 128, 16, dtype)
+    c.k, c.v = c.k[:0], c.v[:0]
     c.check(mcb)
 
 
