@@ -13,6 +13,9 @@ Operator meanings follow the reference:
                                    (src/fusion_emitter_family_a.cpp)
   msm                              @mc.fused Family C, softmax(Q @ K.T) @ V
                                    (src/fusion_emitter_family_c.cpp)
+The operators of a serving step (paged_grow, paged_release, rope, rope_append,
+tree_attention, adjust_logits) have no counterpart there and take torch CUDA
+tensors only.
 """
 from __future__ import annotations
 
@@ -160,14 +163,15 @@ last_result: Result | None = None
 def _call(fn_name, tensors, extra_args, device=-1, flags=0, workspace=None):
     """Calls fn(tensor..., extra..., exec). The descriptors, the execution
     context and the report are packed into one buffer: building the ctypes
-    structures field by field costs about 2 us an operand, packing 0.6 us
-    (12 operands: 29 -> 13 us a call on the host, which is what a small call
+    structures field by field costs about 2 us an operand, packing 0.7 us
+    (10 operands: 25 -> 14 us a call on the host, which is what a small call
     takes)."""
     global last_result
     lib = _abi.load()
     fn, buf, base, ex, rep = _abi.call_frame(fn_name, len(tensors))
     codes = _TORCH_CODE or _torch_codes()
     pack, size = _abi.TENSOR_PACK, _abi.TENSOR_SIZE
+    pack1 = pack[1]
     device_call = False
     at, args = 0, []
     for name, t in tensors:
@@ -175,9 +179,13 @@ def _call(fn_name, tensors, extra_args, device=-1, flags=0, workspace=None):
             args.append(None)
         else:
             try:  # torch tensors, nearly always
-                rank, dev = t.dim(), t.is_cuda
-                pack[rank](buf, at, _abi.ABI_VERSION, size, t.data_ptr(), codes[t.dtype], rank,
-                           *t.shape, *t.stride(), 2 if dev else 1)  # MEM_DEVICE, MEM_HOST
+                shape, dev = t.shape, t.is_cuda
+                if len(shape) == 1:  # (asking for one stride costs as much as all the rest)
+                    pack1(buf, at, 1, size, t.data_ptr(), codes[t.dtype], 1, shape[0],
+                          1 if t.is_contiguous() else t.stride(0), 2 if dev else 1)
+                else:  # ABI_VERSION, ..., MEM_DEVICE or MEM_HOST
+                    pack[len(shape)](buf, at, 1, size, t.data_ptr(), codes[t.dtype], len(shape),
+                                     *shape, *t.stride(), 2 if dev else 1)
             except (KeyError, AttributeError, TypeError, IndexError):
                 d, dev = _desc(t, name)
                 buf[at:at + size] = bytes(d)
