@@ -26,8 +26,8 @@ namespace {
 
 constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
-constexpr int MAX_SPLITS = 64;
-constexpr int MIN_KEYS = 256;  // keys a slice is worth a CTA for
+constexpr int MAX_SPLITS = 64;  // two a lane when they are joined
+constexpr int MIN_KEYS = 128;  // keys a slice is worth a CTA for (64: shorter contexts lose)
 
 template <typename T>
 __device__ __forceinline__ float to_f32(T v) {
@@ -51,8 +51,8 @@ __device__ __forceinline__ int32_t request_of(const TreeAttn &p, int64_t t) {
 // kRows query heads of one token; kCols = elements of a head per lane.
 template <typename T, int kRows, int kCols>
 __global__ void __launch_bounds__(THREADS) tree_attn_simt_kernel(const TreeAttn p, float *partial,
-                                                                 int splits) {
-  extern __shared__ float smem[];
+                                                                 int splits, int vec) {
+  extern __shared__ __align__(16) float smem[];
   float *qs = smem;                                     // [kRows][dim]
   float *red = smem + kRows * p.dim;                    // [WARPS][kRows][dim + 2]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -106,10 +106,29 @@ __global__ void __launch_bounds__(THREADS) tree_attn_simt_kernel(const TreeAttn 
       for (int r = 0; r < kRows; ++r) s[r] = 0.0f;
       if (visible) {
         const T *k = static_cast<const T *>(p.k) + ko;
-        for (int d = 0; d < p.dim; ++d) {
-          const float x = to_f32(k[d]);
+        if (vec) {  // rows that can be read 16 bytes at a time
+          constexpr int VE = 16 / sizeof(T);
+#pragma unroll 8
+          for (int d = 0; d < p.dim; d += VE) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(k + d);
+            const T *x = reinterpret_cast<const T *>(&w);
 #pragma unroll
-          for (int r = 0; r < kRows; ++r) s[r] = fmaf(qs[r * p.dim + d], x, s[r]);
+            for (int e = 0; e < VE; e += 4) {
+              const float x0 = to_f32(x[e]), x1 = to_f32(x[e + 1]);
+              const float x2 = to_f32(x[e + 2]), x3 = to_f32(x[e + 3]);
+#pragma unroll
+              for (int r = 0; r < kRows; ++r) {
+                const float4 q4 = *reinterpret_cast<const float4 *>(qs + r * p.dim + d + e);
+                s[r] = fmaf(q4.w, x3, fmaf(q4.z, x2, fmaf(q4.y, x1, fmaf(q4.x, x0, s[r]))));
+              }
+            }
+          }
+        } else {
+          for (int d = 0; d < p.dim; ++d) {
+            const float x = to_f32(k[d]);
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) s[r] = fmaf(qs[r * p.dim + d], x, s[r]);
+          }
         }
       }
 #pragma unroll
@@ -131,19 +150,29 @@ __global__ void __launch_bounds__(THREADS) tree_attn_simt_kernel(const TreeAttn 
 #pragma unroll
         for (int c = 0; c < kCols; ++c) acc[r][c] *= f;
       }
-      for (uint32_t left = seen; left; left &= left - 1) {
-        const int j = __ffs(left) - 1;
-        const T *v = static_cast<const T *>(p.v) + __shfl_sync(0xffffffffu, vo, j);
-        float w[kRows];
+      // The values of kMany keys on their way at a time; a key that is not seen
+      // is not read and counts 0 x 0.
+      constexpr int kMany = kCols >= 8 ? 4 : 8;
+#pragma unroll 1
+      for (int j0 = 0; j0 < 32; j0 += kMany) {
+        if (((seen >> j0) & ((1u << kMany) - 1)) == 0) continue;
+        float x[kMany][kCols];
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) w[r] = __shfl_sync(0xffffffffu, s[r], j);
+        for (int u = 0; u < kMany; ++u) {
+          const T *v = static_cast<const T *>(p.v) + __shfl_sync(0xffffffffu, vo, j0 + u);
+          const bool bit = (seen >> (j0 + u)) & 1u;
 #pragma unroll
-        for (int c = 0; c < kCols; ++c) {
-          const int d = c * 32 + lane;
-          const float x = d < p.dim ? to_f32(v[d]) : 0.0f;
-#pragma unroll
-          for (int r = 0; r < kRows; ++r) acc[r][c] = fmaf(w[r], x, acc[r][c]);
+          for (int c = 0; c < kCols; ++c)
+            x[u][c] = bit && c * 32 + lane < p.dim ? to_f32(v[c * 32 + lane]) : 0.0f;
         }
+#pragma unroll
+        for (int u = 0; u < kMany; ++u)
+#pragma unroll
+          for (int r = 0; r < kRows; ++r) {
+            const float w = __shfl_sync(0xffffffffu, s[r], j0 + u);
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) acc[r][c] = fmaf(w, x[u][c], acc[r][c]);
+          }
       }
     }
   }
@@ -207,19 +236,34 @@ __global__ void __launch_bounds__(256) tree_attn_join_kernel(const TreeAttn p, c
   const int64_t t = row / p.heads, h = row - t * p.heads;
   const int stride = p.dim + 2;
   const float *in = partial + row * splits * stride;
-  float mx = -INFINITY, sum = 0.0f;
-  for (int z = 0; z < splits; ++z) mx = fmaxf(mx, in[z * stride + p.dim]);
+  // Slices z = lane and lane + 32: their maxima and sums, and what they weigh.
+  float m[2], l[2], w[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int z = lane + 32 * u;
+    m[u] = z < splits ? in[z * stride + p.dim] : -INFINITY;
+    l[u] = z < splits ? in[z * stride + p.dim + 1] : 0.0f;
+  }
+  float mx = fmaxf(m[0], m[1]);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
   const float ref = mx == -INFINITY ? 0.0f : mx;
-  for (int z = 0; z < splits; ++z)
-    sum += in[z * stride + p.dim + 1] * expf(in[z * stride + p.dim] - ref);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) w[u] = expf(m[u] - ref);
+  float sum = l[0] * w[0] + l[1] * w[1];
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   T *o = static_cast<T *>(p.o) + t * p.o_s[0] + h * p.o_s[1];
-  for (int d = lane; d < p.dim; d += 32) {
+  for (int d0 = 0; d0 < p.dim; d0 += 32) {
+    const int d = d0 + lane;
     float x = 0.0f;
-    for (int z = 0; z < splits; ++z)
-      if (in[z * stride + p.dim + 1] != 0.0f)
-        x = fmaf(in[z * stride + d], expf(in[z * stride + p.dim] - ref), x);
-    o[d] = static_cast<T>(x * inv);
+#pragma unroll 8
+    for (int z = 0; z < splits; ++z) {
+      const float f = __shfl_sync(0xffffffffu, z < 32 ? w[0] : w[1], z & 31);
+      x = fmaf(d < p.dim ? in[z * stride + d] : 0.0f, f, x);
+    }
+    if (d < p.dim) o[d] = static_cast<T>(x * inv);
   }
   if (lane == 0 && p.lse)
     p.lse[t * p.lse_s + h] = sum == 0.0f ? -INFINITY : ref + logf(sum);
@@ -248,8 +292,11 @@ cudaError_t run(const TreeAttn &p, float *scratch, int splits, cudaStream_t stre
                   static_cast<unsigned>(splits));
   const size_t smem = sizeof(float) * (kRows * p.dim + WARPS * kRows * (p.dim + 2));
   static_assert(sizeof(float) * (8 * 256 + WARPS * 8 * 258) <= 48 * 1024, "no opt-in needed");
+  constexpr int VE = 16 / sizeof(T);
+  const bool vec = reinterpret_cast<uintptr_t>(p.k) % 16 == 0 &&
+                   (p.dim | p.k_s[0] | p.k_s[1] | p.k_s[2]) % VE == 0;
   tree_attn_simt_kernel<T, kRows, kCols><<<grid, THREADS, smem, stream>>>(
-      p, splits > 1 ? scratch : nullptr, splits);
+      p, splits > 1 ? scratch : nullptr, splits, vec ? 1 : 0);
   if (splits > 1)
     tree_attn_join_kernel<T><<<static_cast<unsigned>((p.tokens * p.heads + 7) / 8), 256, 0,
                                stream>>>(p, scratch, splits);
