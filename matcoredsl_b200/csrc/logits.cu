@@ -11,13 +11,20 @@
 // is cut into slices of the vocabulary; a CTA counts the row's tokens that fall
 // into its slice in shared memory (one word a vocabulary entry: bit 31 "in the
 // prompt", bit 30 "biased", the rest the generated count; integer atomics, so the
-// result does not depend on their order), then finishes the slice. Which of several
-// biases of an entry is the last one is settled there, too, by an atomic maximum. A thread's logits and mask
-// words are loaded before the counting, which then hides their latency. Each
-// slice reads the row's whole history again, from L2. (Clusters of 8 slices that
-// share the reading, each CTA counting a part of the tokens in the others' shared
-// memory, were slower: 96 us against 72 for 256 rows of 131072 with up to 8192
-// tokens, the cluster's barriers costing more than the reading.)
+// result does not depend on their order), then finishes the slice. Which of
+// several biases of an entry is the last one is settled there, too, by an atomic
+// maximum. A thread's logits and mask words are loaded before the counting, which
+// then hides their latency. Each slice reads the row's whole history again, from L2.
+//
+// 256 rows of 131072 bf16 logits to f32, histories of up to 8192 tokens, 300 biases
+// and a mask: 64 us, 210 MB at 3.3 TB/s; without histories 49 us, without biases 47.
+// The reading of the history costs 15 us, the rest is a CTA's load, mark and store
+// following one another with three CTAs to a processor. Measured against it:
+// clusters of 8 slices that share the reading, each CTA counting a part of the
+// tokens in the others' shared memory, 96 us (of 72 then); the tokens sorted by
+// slice in a launch before, 70 us, and 29 against 21 at 64 rows; slices of 4096 with
+// 256 threads 72 us (42 without histories and biases, but twice the reading); 1024
+// threads 86 us, four CTAs of 32 registers 74 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

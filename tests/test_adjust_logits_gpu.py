@@ -69,6 +69,22 @@ def test_logits(mcb, rows, vocab, history, biases, dtype, out_dtype):
     check(mcb, make(rows, vocab, history, biases), dtype, out_dtype)
 
 
+@pytest.mark.parametrize("rows,vocab,history,dtype,pad", [
+    (40, 50001, 20000, "bf16", 0), (3, 131072, 65000, "f32", 0), (300, 16385, 5000, "f16", 1)])
+def test_long_histories(mcb, rows, vocab, history, dtype, pad):
+    """Histories read in many rounds by every slice, some ids outside the vocabulary, a row
+    without any."""
+    c = make(rows, vocab, history, 5)
+    c["ids"][::97] = -1
+    c["ids"][5::97] = vocab + np.arange(len(c["ids"][5::97]))
+    c["ids"][9::31] = vocab - 1
+    cu = c["cu"].copy()
+    cu[1] = 0  # row 0 has none, row 1 takes them
+    c["cu"], c["prompt"][0] = cu, 0
+    check(mcb, c, dtype, "f32", pad=pad)
+    check(mcb, c, dtype, "f32", ("fre",), pad=pad)
+
+
 @pytest.mark.parametrize("use", [(), ("rep",), ("pre",), ("fre",), ("bias",), ("allowed",),
                                  ("rep", "bias")])
 def test_parts(mcb, use):
