@@ -684,9 +684,10 @@ MCB_API mcb_status mcb_rope_append_v1(const mcb_tensor *q_out, const mcb_tensor 
  * q, o and the caches share one type (bf16, f16, f32), dim <= 256. bf16 and
  * f16 with dim 64 or 128, 16-byte aligned bases and strides and a scale other
  * than 0 run on tensor cores (the weights rounded to the 16-bit type for the
- * second product, statistics and sums in f32): requests of up to 32 rows (new
- * tokens x heads per key head) on average on 16-row tiles
- * ("tree_attention_few_rows"), more on tcgen05 ("tcgen05_tree_attention"). All
+ * second product, statistics and sums in f32): requests of few rows (new tokens
+ * x heads per key head; up to 16 on average, or 32 where the table holds at
+ * most 2048 keys; 12 and 24 where T is not the number of requests) on 16-row
+ * tiles ("tree_attention_few_rows"), more on tcgen05 ("tcgen05_tree_attention"). All
  * else runs on CUDA cores in f32 ("simt_tree_attention"). Any block size is
  * taken; powers of two from 8 to 128 and multiples of 128 are copied by TMA on
  * the first route. Scratch for partial results of contexts that several CTAs

@@ -334,7 +334,6 @@ cudaError_t launch_tree_attn_tc(const TreeAttn &p, int dtype, void *scratch, uin
                                 int sms, cudaStream_t stream, LaunchInfo *info);
 
 // ---- tree_attn_few.cu: the same for requests of few rows --------------------------------------
-constexpr int64_t kTreeFewRows = 32;  // rows (new tokens x group) of a request, on average
 bool tree_attn_few_ok(const TreeAttn &p, int dtype);
 uint64_t tree_attn_few_scratch(const TreeAttn &p, int sms);
 cudaError_t launch_tree_attn_few(const TreeAttn &p, int dtype, void *scratch, uint32_t *status,

@@ -1,5 +1,5 @@
 // Attention of drafted tokens over a paged cache for requests of few rows (a
-// row = new token x query heads of the group), up to 32: bf16 or f16,
+// row = new token x query heads of the group), up to 16, with short contexts 32: bf16 or f16,
 // head size 64 or 128, 16-byte aligned rows. (The mathematics and the masks:
 // tree_attn.cu; how the work is shared out: tree_attn.cuh.)
 //
@@ -595,10 +595,20 @@ __global__ void __launch_bounds__(threads<kTma>())
   }
 }
 
-// Row tiles of 16 that a CTA takes: by the rows that a request has on average.
+// Row tiles of 16 that a CTA takes, 0 where tcgen05 is the faster. By the rows that a
+// request has on average; of drafted tokens some requests have more than that, and
+// one whose rows do not fit reads its context twice, so a tile counts as 12 rows then.
+//   one tile: 64 requests of 4 rows, up to 8192 keys 189 us (304 on tcgen05, 230 with two
+//     tiles); 32 of 16 rows 102 (112); of 9 to 20 rows 243 (221), hence 12.
+//   two tiles: 256 requests of 16 to 32 rows, up to 1000 keys 183 us (225 on tcgen05, whose
+//     units cost three tiles more than their keys), 2000 keys 288 (317), 4000 keys 487
+//     (461); 64 requests with 4000 keys 142 (125), 8192 keys 245 (228); of 20 to 40 rows
+//     with 1000 keys 74 (68). So they are taken where no context can pass 2048 keys.
 int row_tiles(const TreeAttn &a) {
   const int64_t rows = a.tokens * (a.heads / a.kv_heads);
-  return rows <= 16 * a.requests ? 1 : 2;
+  const int64_t tile = a.tokens == a.requests ? 16 : 12;
+  if (rows <= tile * a.requests) return 1;
+  return rows <= 2 * tile * a.requests && a.columns * a.block <= 2048 ? 2 : 0;
 }
 template <int HD, int MT>
 constexpr int per_sm() {  // CTAs that fit into an SM's shared memory (228 KB, 1 KB kept per CTA)
@@ -664,8 +674,7 @@ cudaError_t run_rows(const TreeAttn &a, void *scratch, uint32_t *status, int sms
 }  // namespace
 
 bool tree_attn_few_ok(const TreeAttn &a, int dtype) {
-  return tree_attn_tc_ok(a, dtype) &&
-         a.tokens * (a.heads / a.kv_heads) <= kTreeFewRows * a.requests;
+  return tree_attn_tc_ok(a, dtype) && row_tiles(a) > 0;
 }
 
 uint64_t tree_attn_few_scratch(const TreeAttn &a, int sms) {

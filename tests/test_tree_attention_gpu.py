@@ -91,6 +91,9 @@ SHAPES = [  # new, kv, heads, kv_heads, dim, block
     ([130], [400], 4, 2, 128, 128),
     ([7], [3000], 16, 1, 128, 48),
     ([9, 1], [20, 2500], 40, 8, 128, 1),
+    ([7, 1], [20, 1900], 40, 8, 128, 1),
+    ([1] * 9, [i * 250 for i in range(9)], 32, 1, 128, 16),
+    ([4, 2, 9], [900, 2, 2000], 16, 4, 64, 40),
     ([3], [1000], 8, 2, 64, 256),
     ([33], [700], 8, 2, 128, 256)]
 
@@ -100,8 +103,11 @@ SHAPES = [  # new, kv, heads, kv_heads, dim, block
 @pytest.mark.parametrize("tree", [True, False])
 def test_sixteen_bits(mcb, shape, dtype, tree):
     new, _, heads, kv_heads = shape[:4]
-    few = sum(new) * (heads // kv_heads) <= 32 * len(new)
-    Case(*shape, dtype, tree).check(
+    c = Case(*shape, dtype, tree)
+    rows, n = sum(new) * (heads // kv_heads), len(new)
+    tile = 16 if sum(new) == n else 12
+    few = rows <= tile * n or (rows <= 2 * tile * n and c.table.shape[1] * shape[5] <= 2048)
+    c.check(
         mcb, "tree_attention_few_rows" if few else "tcgen05_tree_attention")
 
 
