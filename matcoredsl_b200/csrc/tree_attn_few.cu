@@ -6,7 +6,7 @@
 // Bound: reading the cache. With R rows a key and value row of 4 * HD bytes
 // take 4 * HD * R operations, far below what a CTA can do in the time of the
 // read, so the kernel is built around the copies: six half tiles (128 keys or
-// values, 32 KiB at HD = 128) are in shared memory or on their way. The products
+// values, 32 KiB at HD = 128) of an SM are in shared memory or on their way. The products
 // use warp-level matrix instructions on 16-row tiles: the 128-row tile of a
 // tcgen05 instruction would be empty but for a few rows, and its softmax would
 // run on one warp.
@@ -40,7 +40,12 @@ template <bool kTma>
 constexpr int threads() {
   return COMPUTE + 32 + (kTma ? 0 : COPIERS);
 }
-constexpr int HALVES = 6;  // half tiles (keys or values) in shared memory
+// Half tiles (keys or values) in shared memory. With 3 of head size 128 two CTAs fit
+// into an SM, with one CTA they are 1% slower than 6.
+template <int HD, int MT, bool kTma>
+constexpr int halves() {
+  return HD == 128 && MT == 1 && kTma ? 3 : 6;
+}
 constexpr int TILES = 4;   // ring of prepared tiles
 constexpr int QBUFS = 2;
 
@@ -51,8 +56,9 @@ struct Tile {
   int32_t tile;        // of the segment
 };
 
-template <int HD, int MT>
+template <int HD, int MT, bool kTma>
 struct Smem {
+  static constexpr int HALVES = halves<HD, MT, kTma>();
   uint8_t kv[HALVES][BK * HD * 2];
   uint8_t q[QBUFS][16 * MT * HD * 2];
   uint8_t p[16 * MT * BK * 2];  // weights; maxima and sums of the warps in between
@@ -63,7 +69,7 @@ struct Smem {
   int32_t start_w;
   int abort_flag, dirty;
 };
-static_assert(sizeof(Smem<128, 2>) <= 232448, "exceeds the shared memory per block");
+static_assert(sizeof(Smem<128, 2, true>) <= 232448, "exceeds the shared memory per block");
 
 struct Params : TreeParams {
   float sign;         // of the scale
@@ -128,7 +134,8 @@ __global__ void __launch_bounds__(threads<kTma>())
   constexpr int PIECES = HD / 8;  // 16-byte pieces of a key, value or query row
   constexpr int NT = HD / 64;     // 8-column tiles of O per warp
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  Smem<HD, MT> &sm = *reinterpret_cast<Smem<HD, MT> *>(smem_raw);
+  constexpr int HALVES = halves<HD, MT, kTma>();
+  Smem<HD, MT, kTma> &sm = *reinterpret_cast<Smem<HD, MT, kTma> *>(smem_raw);
   const TreeAttn &a = p.a;
   volatile int *abort_flag = &sm.abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -610,9 +617,15 @@ int row_tiles(const TreeAttn &a) {
   if (rows <= tile * a.requests) return 1;
   return rows <= 2 * tile * a.requests && a.columns * a.block <= 2048 ? 2 : 0;
 }
-template <int HD, int MT>
-constexpr int per_sm() {  // CTAs that fit into an SM's shared memory (228 KB, 1 KB kept per CTA)
-  return 2 * (sizeof(Smem<HD, MT>) + 1024) <= 233472 ? 2 : 1;
+// CTAs per SM: two where they fit (228 KB of shared memory, 1 KB kept per CTA) and there
+// are enough units, else contexts are cut into more parts than the second CTA is worth.
+// Head size 128, 8 key heads, up to 8192 keys: 1 request 26.6 us with one, 35.4 with two;
+// 32 requests 99.4 both; 64 requests 187 and 181, up to 1000 keys 43 and 37. Head size
+// 64: 1 request 24.6 and 32.3, 4 requests 25.1 and 27.0, 8 requests 32.7 and 29.0.
+template <int HD, int MT, bool kTma>
+int per_sm(const TreeAttn &a, int sms) {
+  if (2 * (sizeof(Smem<HD, MT, kTma>) + 1024) > 233472) return 1;
+  return a.requests * a.kv_heads >= (HD == 128 ? 2 * sms : sms / 4) ? 2 : 1;
 }
 
 // Rows of a TMA box, 0 where blocks are no whole boxes.
@@ -636,13 +649,13 @@ bool cache_map(CUtensorMap *map, const TreeAttn &a, const void *base, const int6
 template <int HD, int MT, bool kF16, bool kTma>
 cudaError_t run(const TreeAttn &a, const CUtensorMap &tk, const CUtensorMap &tv, void *scratch,
                 uint32_t *status, int sms, cudaStream_t stream, LaunchInfo *info) {
-  const int ctas = sms * per_sm<HD, MT>();
+  const int ctas = sms * per_sm<HD, MT, kTma>(a, sms);
   Params p;
   static_cast<TreeParams &>(p) = tree_params(a, scratch, 16 * MT, ctas, status);
   p.sign = a.scale < 0.0f ? -1.0f : 1.0f;
   p.page_rows = kTma ? page_rows(a) : BK;
   auto kernel = tree_attn_few_kernel<HD, MT, kF16, kTma>;
-  constexpr int smem = static_cast<int>(sizeof(Smem<HD, MT>));
+  constexpr int smem = static_cast<int>(sizeof(Smem<HD, MT, kTma>));
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
@@ -651,7 +664,7 @@ cudaError_t run(const TreeAttn &a, const CUtensorMap &tk, const CUtensorMap &tv,
   info->tile_m = 16 * MT;
   info->tile_n = BK;
   info->tile_k = HD;
-  info->stages = HALVES;
+  info->stages = halves<HD, MT, kTma>();
   info->ctas = ctas;
   info->set_route("tree_attention_few_rows");
   return launch_join<HD, 16 * MT, kF16>(p, ctas, stream);
@@ -679,8 +692,8 @@ bool tree_attn_few_ok(const TreeAttn &a, int dtype) {
 
 uint64_t tree_attn_few_scratch(const TreeAttn &a, int sms) {
   const bool one = row_tiles(a) == 1;
-  const int n = a.dim == 128 ? (one ? per_sm<128, 1>() : per_sm<128, 2>())
-                             : (one ? per_sm<64, 1>() : per_sm<64, 2>());
+  const int n = a.dim == 128 ? (one ? per_sm<128, 1, true>(a, sms) : per_sm<128, 2, true>(a, sms))
+                             : (one ? per_sm<64, 1, true>(a, sms) : per_sm<64, 2, true>(a, sms));
   return tree_scratch(a, one ? 16 : 32, n * sms);
 }
 
