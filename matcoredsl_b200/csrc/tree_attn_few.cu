@@ -24,7 +24,8 @@
 // each key of a tile lies and copies the queries and, where a cache block is a
 // whole box of a tensor map (8 rows or more, and a divisor or multiple of 128),
 // keys and values by TMA. Blocks of other sizes are copied row by row with
-// cp.async by eight more warps. (The compute warps issuing those copies themselves,
+// cp.async by eight more warps: 64 requests of up to 8192 keys take 211 us with blocks of
+// 24, 180 with blocks of 16 (1.09 GB at 6.1 TB/s). (The compute warps issuing those copies themselves,
 // between their products, took 2.4 us a tile: 1.6 thousand cycles of the copies'
 // own.)
 #include "tree_attn.cuh"
@@ -35,7 +36,7 @@ using namespace tree;
 
 constexpr int WARPS = 8;
 constexpr int COMPUTE = WARPS * 32;
-constexpr int COPIERS = 256;  // threads of the row-by-row copies (128: 270 us where they take 205)
+constexpr int COPIERS = 256;  // threads of the row-by-row copies (128: 270 us where these take 211)
 template <bool kTma>
 constexpr int threads() {
   return COMPUTE + 32 + (kTma ? 0 : COPIERS);
