@@ -120,6 +120,47 @@ def test_any_size(mcb, shape, dtype, tree):
     Case(*shape, dtype, tree).check(mcb)
 
 
+@pytest.mark.parametrize("shape", [
+    ([40, 0, 1, 70, 33, 3, 5], [40, 0, 900, 75, 300, 2, 64], 8, 4, 128, 16),
+    ([9] * 70, [9 + 7 * i for i in range(70)], 1, 1, 80, 24), ([2] * 200, [50] * 200, 4, 2, 33, 8),
+    ([150, 160, 1], [1500, 161, 3], 3, 1, 256, 64), ([5, 2] * 40, [33, 90] * 40, 20, 4, 64, 16)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("tree", [True, False])
+def test_any_size_many_tokens(mcb, shape, dtype, tree):
+    """Enough tokens for several of them to share a CTA, across the borders of requests."""
+    c = Case(*shape, dtype, tree)
+    if tree:
+        bits = c.bits.copy()
+        bits[::11] = False
+        c.set_bits(bits)
+    c.check(mcb)
+
+
+@pytest.mark.parametrize("heads", [2, 6])
+def test_many_tokens_do_not_see_each_others_values(mcb, heads):
+    """Infinities in the values of some drafts, in f32: they reach the rows that see them, no other."""
+    import torch
+    new = [7, 3, 12, 30] * 10
+    c = Case(new, [n + 20 for n in new], heads, 2, 128, 16, "f32")
+    hit = {}
+    for b in range(0, 40, 3):
+        j = new[b] // 2
+        pos = 20 + j
+        c.v[int(c.table[b, pos // 16]), pos % 16, :, ::3] = float("inf")
+        hit[b] = j
+    i32 = lambda a: torch.from_numpy(np.ascontiguousarray(a)).int().cuda()  # noqa: E731
+    got = mcb.tree_attention(c.q, c.k, c.v, i32(c.table), i32(c.cu), i32(c.kv), i32(c.mask))
+    assert mcb.api.last_result.route == "simt_tree_attention"
+    got = got.cpu().numpy()
+    for b in range(40):
+        for t in range(c.cu[b], c.cu[b + 1]):
+            if b in hit and c.bits[t, hit[b]]:
+                assert np.isposinf(got[t, :, ::3]).all()
+            else:
+                assert np.isfinite(got[t, :, ::3]).all()
+            assert np.isfinite(np.delete(got[t], np.s_[::3], 1)).all()
+
+
 def test_large_scores(mcb):
     """Scores whose largest grows along the keys, far past where a first maximum would overflow."""
     for dtype in ("bf16", "f32"):
