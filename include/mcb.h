@@ -165,10 +165,12 @@ MCB_API mcb_status mcb_device_status(int32_t device, uint32_t *word, int32_t cle
  * adapter's poison domain (compiler/lib/runtime/closed_cuda_candidate_v1.cpp:86-120):
  * runs one tensor-core GEMM tile on `device` whose loads are never issued,
  * so its pipeline wait gives up after `spin_limit_cycles` (10^4..4*10^9
- * clock64 cycles; ordinary launches use ~2 s). Returns
- * MCB_STATUS_DEVICE_TIMEOUT when the kernel returned and reported the stall
- * (bit 0, "producer data never arrived", set in the device status word,
- * which stays set until cleared with mcb_device_status). Synchronises the
+ * clock64 cycles; ordinary launches use ~2 s), then a wait of the kind that
+ * ends the kernels (no other role can cut it short) on a phase that never
+ * completes. Returns MCB_STATUS_DEVICE_TIMEOUT when both kernels returned and
+ * reported their stall (bit 0, "producer data never arrived", and bit 3, "final
+ * tensor-core drain stalled", set in the device status word, which stays set
+ * until cleared with mcb_device_status). Synchronises the
  * device; allocates 112 KiB for the call. */
 MCB_API mcb_status mcb_device_timeout_selftest_v1(int32_t device,
                                                   uint64_t spin_limit_cycles) MCB_NOEXCEPT;

@@ -2481,10 +2481,10 @@ MCB_API mcb_status mcb_device_timeout_selftest_v1(int32_t device,
   uint32_t word = 0;
   if (cudaMemcpy(&word, c->status, 4, cudaMemcpyDeviceToHost) != cudaSuccess)
     return MCB_STATUS_CANDIDATE_FAILURE;
-  // The stalled wait must have been reported; the word stays set (sticky)
+  // Both stalled waits must have been reported; the word stays set (sticky)
   // until the caller clears it with mcb_device_status.
-  constexpr uint32_t kTimeoutFullBit = 1u;  // kErrTimeoutFull of the device status word
-  return (word & kTimeoutFullBit) ? MCB_STATUS_DEVICE_TIMEOUT : MCB_STATUS_CANDIDATE_FAILURE;
+  constexpr uint32_t kTimeoutBits = 1u | 1u << 3;  // kErrTimeoutFull, kErrTimeoutDrain of the word
+  return (word & kTimeoutBits) == kTimeoutBits ? MCB_STATUS_DEVICE_TIMEOUT : MCB_STATUS_CANDIDATE_FAILURE;
 }
 
 MCB_API mcb_status mcb_device_peer_timeout_selftest_v1(int32_t device,

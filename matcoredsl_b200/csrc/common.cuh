@@ -70,7 +70,9 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 
 // Wait for the phase with the given parity. Returns false (after recording
 // `err_bit` and raising *abort) if it does not complete within `limit`
-// clock64 cycles or if another role of this CTA already aborted.
+// clock64 cycles or if another role of this CTA already aborted. abort may be
+// null: the wait then only ends by the phase or the limit (the drains of work in
+// flight, which other roles' failures must not cut short).
 __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, volatile int *abort,
                                           uint32_t *status, uint32_t err_bit,
                                           long long limit = kSpinTimeoutCycles) {
@@ -80,10 +82,10 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, volati
   for (uint32_t i = 1;; ++i) {
     if (mbar_try_wait(addr, parity)) return true;
     if ((i & 255u) == 0) {
-      if (*abort) return false;
+      if (abort && *abort) return false;
       if (clock64() - t0 > limit) {
         if (status) atomicOr(status, err_bit);
-        *abort = 1;
+        if (abort) *abort = 1;
         return false;
       }
     }

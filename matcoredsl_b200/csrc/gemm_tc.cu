@@ -1190,11 +1190,22 @@ cudaError_t launch_gemm_tc_bf16(const void *x, const void *w, void *y, int64_t m
   return cudaGetLastError();
 }
 
+// A wait without an abort flag, as the kernels' drains are, on a phase that nothing
+// completes: it must run out after `spin_limit` cycles and record kErrTimeoutDrain.
+__global__ void drain_stall_selftest_kernel(long long spin_limit, uint32_t *status) {
+  __shared__ uint64_t bar;
+  if (threadIdx.x == 0) {
+    mbar_init(&bar, 1);
+    fence_mbar_init();
+    mbar_wait(&bar, 0, nullptr, status, kErrTimeoutDrain, spin_limit);
+  }
+}
+
 // Self-test of the bounded waits: one single-SM GEMM tile (128x64 . 64x256)
 // whose producer issues no loads, so the MMA thread's wait for the first
 // stage must run out after `spin_limit` cycles, record kErrTimeoutFull in
 // *status and abort the CTA (the epilogue warps leave through the abort
-// flag, TMEM is freed). x must hold 128x64 and w 64x256 16-byte-aligned bf16
+// flag, TMEM is freed); then drain_stall_selftest_kernel. x must hold 128x64 and w 64x256 16-byte-aligned bf16
 // elements (they are never read), y 128x256 bf16 (never written).
 cudaError_t launch_gemm_tc_stall_selftest(const void *x, const void *w, void *y,
                                           long long spin_limit, uint32_t *status,
@@ -1223,6 +1234,7 @@ cudaError_t launch_gemm_tc_stall_selftest(const void *x, const void *w, void *y,
                                        static_cast<int>(SMEM_BYTES));
   if (e != cudaSuccess) return e;
   gemm_tc_bf16_kernel<false><<<1, THREADS, SMEM_BYTES, stream>>>(tx, tw, p);
+  drain_stall_selftest_kernel<<<1, 32, 0, stream>>>(spin_limit, status);
   return cudaGetLastError();
 }
 
