@@ -237,6 +237,11 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
         return table[fast_div(key, p.block)];
       };
       int32_t next = entry(0);
+      // Places count over the segments (`tiles` before this one): a loader reads tile x's
+      // numbers for the last time, for its values, before it arrives for the description of
+      // tile x + 2, and the place is written again for tile x + 4, which the
+      // barrier of x + 3 precedes. Counted from 0 in each segment, a loader that ran ahead
+      // would write the next segment's first tile over numbers that another still reads.
       auto describe = [&](int j) -> bool {
         const int key = key0 + j * BK + l;
         const int32_t blk = next;
@@ -244,7 +249,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
         const bool good = key < sg.keys && blk >= 0 && blk < a.blocks;
         const uint32_t col = fast_div(key, p.block);
         const uint32_t off = key - col * a.block;
-        sm.info[j % INFO_RING][(l % STEP) * PASSES + l / STEP] =
+        sm.info[(tiles + j) % INFO_RING][(l % STEP) * PASSES + l / STEP] =
             good ? (static_cast<uint32_t>(blk) << p.row_bits) | off : kNoRow;
         const uint32_t bits = __ballot_sync(0xffffffffu, good);
         if (lane == 0) sm.valid[(tiles + j) % VALID_RING][warp] = bits;
@@ -260,7 +265,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
         const uint32_t dst = smem_u32(sm.kv[s]) + dst0;
         const uint32_t blk_step = p.step[value][0], row_step = p.step[value][1];
         const uint4 *info =
-            reinterpret_cast<const uint4 *>(sm.info[j % INFO_RING]) + r0 * (PASSES / 4);
+            reinterpret_cast<const uint4 *>(sm.info[(tiles + j) % INFO_RING]) + r0 * (PASSES / 4);
 #pragma unroll
         for (int it = 0; it < PASSES; it += 4) {
           const uint4 w = info[it / 4];
