@@ -183,6 +183,12 @@ MCB_API mcb_status mcb_device_timeout_selftest_v1(int32_t device,
  * about 8.3 MiB for the call. */
 MCB_API mcb_status mcb_device_peer_timeout_selftest_v1(int32_t device,
                                                        uint64_t spin_limit_cycles) MCB_NOEXCEPT;
+/* The same for the attention of few rows over a paged cache: one warp of each CTA
+ * behaves as if its wait for a tile's values had run out, at the first (last = 0)
+ * or the last (last = 1) tile of its context. Returns MCB_STATUS_DEVICE_TIMEOUT
+ * when the kernel returned and reported it (bit 0, sticky). Synchronises the
+ * device; allocates about 350 KiB for the call. */
+MCB_API mcb_status mcb_device_tree_timeout_selftest_v1(int32_t device, int32_t last) MCB_NOEXCEPT;
 /* Ok when `device` is an sm_100 GPU this build can run on; replaces
  * detail::cudaCandidateAvailable (compiler/lib/runtime/closed_cuda_candidate_v1.h:13). */
 MCB_API mcb_status mcb_candidate_available(int32_t device) MCB_NOEXCEPT;

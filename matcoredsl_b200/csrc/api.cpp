@@ -2534,6 +2534,69 @@ MCB_API mcb_status mcb_device_peer_timeout_selftest_v1(int32_t device,
   return (word & kTimeoutPeerBit) ? MCB_STATUS_DEVICE_TIMEOUT : MCB_STATUS_CANDIDATE_FAILURE;
 }
 
+MCB_API mcb_status mcb_device_tree_timeout_selftest_v1(int32_t device, int32_t last) noexcept {
+  if (last != 0 && last != 1) return MCB_STATUS_INVALID_ARGUMENT;
+  if (hooks()) return MCB_STATUS_CANDIDATE_UNAVAILABLE;
+  mcb_exec ex{};
+  ex.abi_version = MCB_ABI_VERSION_V1;
+  ex.struct_size = sizeof(ex);
+  ex.device = device;
+  int dev;
+  mcb_status s = resolve_device(&ex, &dev);
+  if (s) return s;
+  DeviceGuard g(dev);
+  if (!g.ok) return MCB_STATUS_CANDIDATE_FAILURE;
+  DeviceCtx *c;
+  if ((s = init_ctx(dev, &c))) return s;
+  // One token of one head of 64 over 1024 keys in blocks of 128, all zero: queries, outputs,
+  // keys, values, then cu_new {0, 1}, the length and the table (blocks 0..7), then scratch.
+  constexpr int kBlocks = 8, kBlock = 128, kDim = 64, kSms = 1;
+  constexpr size_t kRow = 256, kCache = static_cast<size_t>(kBlocks) * kBlock * kDim * 2;
+  mcb::TreeAttn a{};
+  a.tokens = a.requests = 1;
+  a.heads = a.kv_heads = 1;
+  a.dim = kDim;
+  a.block = kBlock;
+  a.q_s[0] = a.q_s[1] = a.o_s[0] = a.o_s[1] = kDim;
+  a.k_s[0] = a.v_s[0] = kBlock * kDim;
+  a.k_s[1] = a.v_s[1] = a.k_s[2] = a.v_s[2] = kDim;
+  a.columns = a.table_stride = a.blocks = kBlocks;
+  a.scale = 1.0f;
+  const size_t used = 3 * kRow + 2 * kCache, all = used + mcb::tree_attn_few_scratch(a, kSms);
+  void *buf = nullptr;
+  if (cudaMalloc(&buf, all) != cudaSuccess) {
+    cudaGetLastError();
+    return MCB_STATUS_ALLOCATION_FAILURE;
+  }
+  uint8_t *base = static_cast<uint8_t *>(buf);
+  const int32_t index[3 + kBlocks] = {0, 1, kBlocks * kBlock, 0, 1, 2, 3, 4, 5, 6, 7};
+  a.q = base;
+  a.o = base + kRow;
+  a.k = base + 3 * kRow;
+  a.v = base + 3 * kRow + kCache;
+  a.cu = reinterpret_cast<int32_t *>(base + 2 * kRow);
+  a.kv_lens = a.cu + 2;
+  a.table = a.cu + 3;
+  cudaError_t err = cudaMemset(base, 0, all);
+  if (err == cudaSuccess)
+    err = cudaMemcpy(base + 2 * kRow, index, sizeof(index), cudaMemcpyHostToDevice);
+  if (err == cudaSuccess)
+    err = mcb::tree_attn_few_ok(a, MCB_DTYPE_BF16)
+              ? mcb::launch_tree_attn_stall_selftest(a, last == 1, base + used, c->status, kSms,
+                                                     nullptr)
+              : cudaErrorInvalidValue;
+  if (err == cudaSuccess) err = cudaDeviceSynchronize();
+  cudaFree(buf);
+  if (err != cudaSuccess) {
+    cudaGetLastError();
+    return MCB_STATUS_CANDIDATE_FAILURE;
+  }
+  uint32_t word = 0;
+  if (cudaMemcpy(&word, c->status, 4, cudaMemcpyDeviceToHost) != cudaSuccess)
+    return MCB_STATUS_CANDIDATE_FAILURE;
+  return (word & 1u) ? MCB_STATUS_DEVICE_TIMEOUT : MCB_STATUS_CANDIDATE_FAILURE;
+}
+
 MCB_API mcb_status mcb_test_set_runtime_hooks_v1(const mcb_runtime_hooks *h) noexcept {
   if (!h) {
     if (g_hooks_on.exchange(false, std::memory_order_acq_rel)) {

@@ -338,6 +338,9 @@ bool tree_attn_few_ok(const TreeAttn &p, int dtype);
 uint64_t tree_attn_few_scratch(const TreeAttn &p, int sms);
 cudaError_t launch_tree_attn_few(const TreeAttn &p, int dtype, void *scratch, uint32_t *status,
                                  int sms, cudaStream_t stream, LaunchInfo *info);
+// Self-test of a wait that runs out (mcb_device_tree_timeout_selftest_v1); see tree_attn_few.cu.
+cudaError_t launch_tree_attn_stall_selftest(const TreeAttn &a, bool last, void *scratch,
+                                            uint32_t *status, int sms, cudaStream_t stream);
 
 // ---- logits.cu: penalties, biases and grammar masks ---------------------------------------------
 struct LogitsParams {

@@ -75,6 +75,7 @@ static_assert(sizeof(Smem<128, 2, true>) <= 232448, "exceeds the shared memory p
 struct Params : TreeParams {
   float sign;         // of the scale
   int32_t page_rows;  // rows of a box (128 without TMA), a power of two
+  int32_t give_up;    // self-test: at a segment's first (0) or last (1) tile
 };
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
@@ -127,7 +128,9 @@ __device__ __forceinline__ uint32_t piece_at(int row, int c, int page) {
   return (row + (row & -page) + (c >> 3) * page) * 128 + swz;
 }
 
-template <int HD, int MT, bool kF16, bool kTma>
+// kTest: one compute warp behaves as if its wait for a tile's values had run out
+// (launch_tree_attn_stall_selftest).
+template <int HD, int MT, bool kF16, bool kTma, bool kTest>
 __global__ void __launch_bounds__(threads<kTma>())
     tree_attn_few_kernel(const __grid_constant__ CUtensorMap tk,
                          const __grid_constant__ CUtensorMap tv, const Params p) {
@@ -306,8 +309,9 @@ __global__ void __launch_bounds__(threads<kTma>())
   const int quad = lane >> 2, ql = lane & 3, page = kTma ? p.page_rows : BK;
   float o[MT][NT][4], ref[MT][2], l[MT][2];
   uint32_t seg_no = 0;
-  // A warp whose wait runs out says so in the tile's barriers with an OR, so that
-  // all warps leave together.
+  // A warp whose wait runs out says so at the tile's next barrier with an OR, and the
+  // warps that found the end come to one, too: all warps leave in the same turn, or a
+  // warp would wait at a barrier for others that have left.
   bool ok = true;
   auto wait = [&](uint64_t *bar, uint32_t parity) {
     ok = mbar_wait_warp(bar, parity, abort_flag, p.status, kErrTimeoutFull) && ok;
@@ -316,7 +320,10 @@ __global__ void __launch_bounds__(threads<kTma>())
     const uint32_t kh = 2 * t, vh = kh + 1;  // half tiles
     wait(&sm.full[t % TILES], (t / TILES) & 1);
     const Tile &d = sm.tile[t % TILES];
-    if (ok && d.seg.kind == kEnd) break;
+    if (ok && d.seg.kind == kEnd) {
+      if (named_bar_or(2, COMPUTE, false)) named_bar_or(1, COMPUTE, false);
+      break;
+    }
     if (ok && d.tile == 0) wait(&sm.q_full[seg_no % QBUFS], (seg_no / QBUFS) & 1);
     if (ok) wait(&sm.kv_full[kh % HALVES], (kh / HALVES) & 1);
     if (!ok) {
@@ -448,7 +455,12 @@ __global__ void __launch_bounds__(threads<kTma>())
         }
       }
     wait(&sm.kv_full[vh % HALVES], (vh / HALVES) & 1);
-    named_bar_sync(3, COMPUTE);  // the weights are there
+    if (kTest && warp == 0 && d.tile == (p.give_up ? sg.ntiles - 1 : 0)) {
+      if (lane == 0) atomicOr(p.status, kErrTimeoutFull);
+      *abort_flag = 1;
+      ok = false;
+    }
+    if (named_bar_or(3, COMPUTE, !ok)) return;  // else the weights are there
     uint8_t *values = sm.kv[vh % HALVES];
     if (drafts) {
       // New tokens' values that are not finite become 0: 0 x inf must not reach
@@ -647,15 +659,17 @@ bool cache_map(CUtensorMap *map, const TreeAttn &a, const void *base, const int6
                         base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int HD, int MT, bool kF16, bool kTma>
+template <int HD, int MT, bool kF16, bool kTma, bool kTest = false>
 cudaError_t run(const TreeAttn &a, const CUtensorMap &tk, const CUtensorMap &tv, void *scratch,
-                uint32_t *status, int sms, cudaStream_t stream, LaunchInfo *info) {
+                uint32_t *status, int sms, cudaStream_t stream, LaunchInfo *info,
+                int give_up = 0) {
   const int ctas = sms * per_sm<HD, MT, kTma>(a, sms);
   Params p;
   static_cast<TreeParams &>(p) = tree_params(a, scratch, 16 * MT, ctas, status);
   p.sign = a.scale < 0.0f ? -1.0f : 1.0f;
   p.page_rows = kTma ? page_rows(a) : BK;
-  auto kernel = tree_attn_few_kernel<HD, MT, kF16, kTma>;
+  p.give_up = give_up;
+  auto kernel = tree_attn_few_kernel<HD, MT, kF16, kTma, kTest>;
   constexpr int smem = static_cast<int>(sizeof(Smem<HD, MT, kTma>));
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -706,6 +720,19 @@ cudaError_t launch_tree_attn_few(const TreeAttn &a, int dtype, void *scratch, ui
                : run_rows<128, false>(a, scratch, status, sms, stream, info);
   return f16 ? run_rows<64, true>(a, scratch, status, sms, stream, info)
              : run_rows<64, false>(a, scratch, status, sms, stream, info);
+}
+
+// Self-test of the way out of a wait that ran out: a call on one row tile of head size 64 in which
+// one warp of each CTA gives up at its segment's first (last = false) or last tile. bf16,
+// blocks of 128; `a` must pass tree_attn_few_ok and its scratch be that of `sms` SMs.
+cudaError_t launch_tree_attn_stall_selftest(const TreeAttn &a, bool last, void *scratch,
+                                            uint32_t *status, int sms, cudaStream_t stream) {
+  CUtensorMap tk{}, tv{};
+  if (a.dim != 64 || row_tiles(a) != 1 || page_rows(a) != BK || !status ||
+      !cache_map(&tk, a, a.k, a.k_s, false, BK) || !cache_map(&tv, a, a.v, a.v_s, false, BK))
+    return cudaErrorInvalidValue;
+  LaunchInfo info;
+  return run<64, 1, false, true, true>(a, tk, tv, scratch, status, sms, stream, &info, last ? 1 : 0);
 }
 
 }  // namespace mcb
