@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(threads<kTma>())
     TreeAttnPart part{};
     Walk<ROWS> walk(p, share, part, sm.start_b, sm.start_w);
     Segment sg;
-    uint32_t count = 0, segs = 0;
+    uint32_t count = 0, segs = 0, armed = 0;  // armed: half tiles that TMA was set to fill
     bool ok = !*abort_flag;
     auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
       ok = __all_sync(0xffffffffu,
@@ -249,6 +249,7 @@ __global__ void __launch_bounds__(threads<kTma>())
             const uint32_t half = 2 * count + value, s = half % HALVES;
             if (!wait(&sm.kv_empty[s], ((half / HALVES) & 1) ^ 1)) break;
             if (lane == 0) mbar_arrive_expect_tx(&sm.kv_full[s], BK * HD * 2);
+            armed = half + 1;
             __syncwarp();
             if (lane < pages)
               tma_load_box(sm.kv[s] + lane * p.page_rows * (HD * 2), value ? &tv : &tk,
@@ -262,6 +263,13 @@ __global__ void __launch_bounds__(threads<kTma>())
     if (ok && slot_free()) {
       if (lane == 0) sm.tile[count % TILES].seg.kind = kEnd;
       mbar_arrive(&sm.full[count % TILES]);
+    }
+    if (!ok) {
+      // Given up: the products did not wait for the copies that are still on their way
+      // into this CTA's shared memory. Each stage's last phase ends them.
+      for (uint32_t s = 0; s < HALVES && s < armed; ++s)
+        mbar_wait(&sm.kv_full[s], ((armed - 1 - s) / HALVES) & 1, nullptr, p.status,
+                  kErrTimeoutDrain);
     }
     cp_async_wait_all();
     if (lane == 0) p.part[blockIdx.x] = part;

@@ -32,6 +32,11 @@ def test_a_wait_that_runs_out_at_the_last_tile(mcb):
     give_up(mcb, 1)
 
 
+def test_a_wait_that_runs_out_while_copies_are_on_their_way(mcb):
+    """The keys and values of the next tiles are being copied: they land before the CTA ends."""
+    give_up(mcb, 0)
+
+
 def test_selftest_refuses_other_places(mcb):
     assert _abi.load().mcb_device_tree_timeout_selftest_v1(0, 2) == \
         _abi.STATUS_CODE["INVALID_ARGUMENT"]
