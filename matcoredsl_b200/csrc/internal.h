@@ -255,7 +255,7 @@ struct FastDiv {
   int32_t shift;
 };
 #if defined(__CUDACC__)
-__device__ __forceinline__ uint32_t fast_div(uint32_t x, const FastDiv &d) {
+__host__ __device__ __forceinline__ uint32_t fast_div(uint32_t x, const FastDiv &d) {
   return static_cast<uint32_t>((static_cast<uint64_t>(x) * d.mul) >> d.shift);
 }
 #endif
@@ -325,7 +325,7 @@ cudaError_t launch_tree_attn_simt(const TreeAttn &p, int dtype, float *scratch, 
 // ---- tree_attn_tc.cu: the same on tcgen05 ------------------------------------------------------
 // A unit of rows whose key tiles lie in several CTAs (left by the first of them).
 struct TreeAttnPart {
-  int32_t parts;  // CTAs it lies in, 0: no such unit starts in this CTA
+  int32_t parts;  // CTAs it lies in, 0: no such unit starts in this CTA, -1: cu_new descends
   int32_t tok0, head, row0, nrows;
 };
 bool tree_attn_tc_ok(const TreeAttn &p, int dtype);

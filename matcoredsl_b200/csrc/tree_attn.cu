@@ -16,7 +16,7 @@
 //
 // Bound: instructions (a value or key element costs a conversion and kRows products a
 // lane), then L2, since every group of rows reads the keys again. f32, 8 requests of
-// up to 8192 keys, 8 key heads of 128, 4 rows each: 130 us, 302 MB at 2.3 TB/s. Several
+// up to 8192 keys, 8 key heads of 128, 4 rows each: 132 us, 302 MB at 2.3 TB/s. Several
 // tokens in a CTA's rows, each with its own visibility, halved 150 causal tokens of one
 // request (72 to 41 us) but cost single tokens 70% (227 us) and drafts 20 to 70%. Two
 // warps a CTA: 146 us (but 121 against 193 for 126 requests of up to 54 keys).
@@ -41,26 +41,18 @@ __device__ __forceinline__ float to_f32(T v) {
   return static_cast<float>(v);
 }
 
-// Number of the request that token t belongs to, -1 when it belongs to none. The
-// warp looks at 32 places at a time: two dependent reads for up to 1024 requests.
-__device__ __forceinline__ int32_t request_of(const TreeAttn &p, int64_t t) {
-  const int lane = threadIdx.x & 31;
-  int64_t lo = 0, n = p.requests;  // the last b of lo .. lo + n - 1 with cu[b] <= t
-  while (n > 1) {
-    const int64_t step = (n + 31) / 32, at = lane * step;
-    const uint32_t le = __ballot_sync(0xffffffffu, at < n && p.cu[lo + at] <= t);
-    const int64_t k = 31 - __clz(le | 1u);
-    lo += k * step;
-    n = min(step, n - k * step);
-  }
-  if (p.requests == 0 || t < p.cu[lo] || t >= p.cu[lo + 1]) return -1;
-  return static_cast<int32_t>(lo);
+// CTAs an SM whose registers the compiler keeps to, 0: its own choice. f32, four heads of up to 128: 5 (without,
+// decoding of 8 requests 141 us instead of 132, of 64 696 instead of 627). The same bound in
+// 16 bits: 16 requests of head size 80 123 us instead of 95.
+template <typename T, int kRows, int kCols>
+constexpr int min_ctas() {
+  return sizeof(T) == 4 && kRows == 4 && kCols == 4 ? 5 : 0;
 }
 
 // kRows query heads of one token; kCols = elements of a head per lane.
 template <typename T, int kRows, int kCols>
-__global__ void __launch_bounds__(THREADS) tree_attn_simt_kernel(const TreeAttn p, float *partial,
-                                                                 int splits, int vec) {
+__global__ void __launch_bounds__(THREADS, min_ctas<T, kRows, kCols>())
+    tree_attn_simt_kernel(const TreeAttn p, float *partial, int splits, int vec) {
   extern __shared__ __align__(16) float smem[];
   float *qs = smem;                                     // [kRows][dim]
   float *red = smem + kRows * p.dim;                    // [WARPS][kRows][dim + 2]
@@ -72,11 +64,27 @@ __global__ void __launch_bounds__(THREADS) tree_attn_simt_kernel(const TreeAttn 
   const int rows = min(kRows, group - g0);
   const int h0 = hk * group + g0;  // first query head
   const T *q = static_cast<const T *>(p.q) + t * p.q_s[0] + h0 * p.q_s[1];
+  // The request that token t belongs to, looked for by all threads while the query is read.
+  // Where cu_new descends, no token belongs to a request; that is why all of it is read and
+  // not searched (for 2000 requests of up to 30 keys, f32, two heads of 64, 24 us
+  // instead of 20.5; nothing to see at 100 requests or 100 keys).
+  __shared__ int32_t owner;
+  int32_t mine = -1;
+  bool descends = false;
+#pragma unroll 4
+  for (int64_t r = threadIdx.x; r < p.requests; r += THREADS) {
+    const int32_t c0 = p.cu[r], c1 = p.cu[r + 1];
+    descends |= c1 < c0;
+    if (c0 <= t && t < c1) mine = static_cast<int32_t>(r);
+  }
+  if (threadIdx.x == 0) owner = -1;
   for (int i = threadIdx.x; i < kRows * p.dim; i += THREADS) {
     const int r = i / p.dim, d = i - r * p.dim;
     qs[i] = r < rows ? to_f32(q[r * p.q_s[1] + d]) * p.scale : 0.0f;
   }
   __syncthreads();
+  if (mine >= 0) owner = mine;
+  descends = __syncthreads_or(descends) != 0;
   float m[kRows], l[kRows], acc[kRows][kCols];
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
@@ -85,7 +93,7 @@ __global__ void __launch_bounds__(THREADS) tree_attn_simt_kernel(const TreeAttn 
 #pragma unroll
     for (int c = 0; c < kCols; ++c) acc[r][c] = 0.0f;
   }
-  const int32_t b = request_of(p, t);
+  const int32_t b = __shfl_sync(0xffffffffu, descends ? -1 : owner, 0);
   if (b >= 0) {
     const int64_t i = t - p.cu[b], n = p.cu[b + 1] - p.cu[b];
     const int64_t kv = max(0, p.kv_lens[b]), prefix = kv - n;

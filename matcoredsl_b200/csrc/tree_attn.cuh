@@ -11,6 +11,10 @@
 // unit that lies in one CTA is finished there; the parts of a unit that spans
 // CTAs go to scratch (at most two per CTA) and a second launch joins them in
 // their order.
+//
+// The arithmetic of the shares is 32-bit; tree_attn_tc_ok() bounds it for requests that
+// share no token. Where cu_new descends somewhere they may, so then nothing is
+// shared out: no token belongs to a request.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -78,8 +82,9 @@ __device__ __forceinline__ void cp_async_wait_all() {
 // One request's lengths, clipped to the tensors.
 struct Request {
   int32_t tok0, rows, prefix, keys;  // rows: of the tokens inside [0, T)
+  bool descends;                     // cu_new does, at this request
 };
-__device__ __forceinline__ Request load_request(const TreeParams &p, int64_t b) {
+__host__ __device__ __forceinline__ Request load_request(const TreeParams &p, int64_t b) {
   const TreeAttn &a = p.a;
   Request r;
   const int64_t c0 = a.cu[b], c1 = a.cu[b + 1], kv = max(0, a.kv_lens[b]);
@@ -89,12 +94,14 @@ __device__ __forceinline__ Request load_request(const TreeParams &p, int64_t b) 
   r.rows = static_cast<int32_t>(in) * p.heads_per_kv;
   r.prefix = static_cast<int32_t>(kv - n);
   r.keys = static_cast<int32_t>(min(kv, static_cast<int64_t>(p.most_keys)));
+  r.descends = c1 < c0;
   return r;
 }
 // Key tiles of row tile `rt`: without a mask the rows see no key past the
 // last one's own.
 template <int ROWS>
-__device__ __forceinline__ int32_t unit_tiles(const TreeParams &p, const Request &r, int32_t rt) {
+__host__ __device__ __forceinline__ int32_t unit_tiles(const TreeParams &p, const Request &r,
+                                                       int32_t rt) {
   int32_t end = r.keys;
   if (!p.a.mask) {
     const int32_t last = min(r.rows, (rt + 1) * ROWS) - 1;
@@ -107,11 +114,11 @@ __device__ __forceinline__ int32_t unit_tiles(const TreeParams &p, const Request
 // 32 rows: 1 (2 and 3 made decoding of 64 requests with up to 1000 keys 3 and 10%
 // slower); 128 or 256 rows: 3 (1 made 24 wide trees 15% slower).
 template <int ROWS>
-constexpr int32_t unit_cost() {
+__host__ __device__ constexpr int32_t unit_cost() {
   return ROWS <= 32 ? 1 : 3;
 }
 template <int ROWS>
-__device__ __forceinline__ int32_t head_cost(const TreeParams &p, const Request &r) {
+__host__ __device__ __forceinline__ int32_t head_cost(const TreeParams &p, const Request &r) {
   const int32_t rts = (r.rows + ROWS - 1) / ROWS;
   if (p.a.mask) return rts ? rts * (unit_tiles<ROWS>(p, r, 0) + unit_cost<ROWS>()) : 0;
   int32_t sum = 0;
@@ -136,48 +143,70 @@ __device__ __forceinline__ uint32_t visible_word(const TreeAttn &a, const uint32
   return s ? (lo >> s) | (word((j >> 5) + 1) << (32 - s)) : lo;
 }
 
-// This CTA's share [w0, w1) of all units' costs, found by all THREADS threads of it
-// (`scan`: THREADS / 32 words of shared memory), and where the requests that hold
-// w0 begin. The first `extra` CTAs take share + 1, the others share.
+// CTA `cta`'s share [w0, w1) of all units' costs. The first `extra` CTAs take
+// share + 1, the others share.
 struct Share {
-  int32_t w0, w1, share, extra;
+  int32_t w0, w1, share, extra, cta;
+  bool descends;  // cu_new does: nothing is shared out
 };
-template <int ROWS, int THREADS>
-__device__ __forceinline__ Share find_share(const TreeParams &p, int32_t *scan, bool usable,
-                                            int64_t *start_b, int32_t *start_w) {
-  const TreeAttn &a = p.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t per_thread = (a.requests + THREADS - 1) / THREADS;
-  const int64_t b_first = threadIdx.x * per_thread;
-  const int64_t b_last = min(a.requests, b_first + per_thread);
-  int32_t mine = 0;
-  for (int64_t b = b_first; b < b_last; ++b)
-    mine += head_cost<ROWS>(p, load_request(p, b)) * a.kv_heads;
-  int32_t incl = mine;
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const int32_t o = __shfl_up_sync(0xffffffffu, incl, off);
-    if (lane >= off) incl += o;
-  }
-  if (lane == 31) scan[warp] = incl;
-  __syncthreads();
-  int32_t total = 0, before = incl - mine;
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) {
-    if (w < warp) before += scan[w];
-    total += scan[w];
-  }
-  const int32_t cta = blockIdx.x, ctas = min(static_cast<int32_t>(gridDim.x), total);
+__host__ __device__ __forceinline__ Share share_of(int32_t cta, int32_t grid, int32_t total,
+                                                   bool usable, bool descends) {
+  const int32_t ctas = descends ? 0 : min(grid, total);
   const bool works = cta < ctas && usable;
   Share s;
   s.share = works ? total / ctas : 0;
   s.extra = works ? total - s.share * ctas : 0;
   s.w0 = cta * s.share + min(cta, s.extra);
   s.w1 = works ? s.w0 + s.share + (cta < s.extra) : s.w0;
+  s.cta = cta;
+  s.descends = descends;
+  return s;
+}
+// Costs of the requests b0 .. b1 - 1, up to one at which cu_new descends.
+template <int ROWS>
+__host__ __device__ __forceinline__ uint32_t requests_cost(const TreeParams &p, int64_t b0,
+                                                           int64_t b1, bool &descends) {
+  uint32_t sum = 0;
+  for (int64_t b = b0; b < b1 && !descends; ++b) {
+    const Request r = load_request(p, b);
+    descends = r.descends;
+    sum += static_cast<uint32_t>(head_cost<ROWS>(p, r)) * static_cast<uint32_t>(p.a.kv_heads);
+  }
+  return sum;
+}
+
+// This CTA's share, found by all THREADS threads of it (`scan`: THREADS / 32 words of
+// shared memory), and where the requests that hold w0 begin.
+template <int ROWS, int THREADS>
+__device__ __forceinline__ Share find_share(const TreeParams &p, uint32_t *scan, bool usable,
+                                            int64_t *start_b, int32_t *start_w) {
+  const TreeAttn &a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t per_thread = (a.requests + THREADS - 1) / THREADS;
+  const int64_t b_first = threadIdx.x * per_thread;
+  bool descends = false;
+  const uint32_t mine =
+      requests_cost<ROWS>(p, b_first, min(a.requests, b_first + per_thread), descends);
+  uint32_t incl = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const uint32_t o = __shfl_up_sync(0xffffffffu, incl, off);
+    if (lane >= off) incl += o;
+  }
+  if (lane == 31) scan[warp] = incl;
+  descends = __syncthreads_or(descends) != 0;
+  uint32_t total = 0, before = incl - mine;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += scan[w];
+    total += scan[w];
+  }
+  const Share s = share_of(blockIdx.x, gridDim.x, static_cast<int32_t>(total), usable, descends);
   // The thread whose requests hold w0 leaves where they begin.
-  if (works && before <= s.w0 && s.w0 < before + mine) {
+  const uint32_t w0 = static_cast<uint32_t>(s.w0);
+  if (s.w0 < s.w1 && before <= w0 && w0 < before + mine) {
     *start_b = b_first;
-    *start_w = before;
+    *start_w = static_cast<int32_t>(before);
   }
   __syncthreads();
   return s;
@@ -194,9 +223,10 @@ struct Walk {
   int64_t b;
   int32_t w, head = 0, rt = 0, n = 0, at = 0;  // at: place within the unit of n tiles
 
-  __device__ __forceinline__ Walk(const TreeParams &args, const Share &share, TreeAttnPart &first,
+  __host__ __device__ __forceinline__ Walk(const TreeParams &args, const Share &share, TreeAttnPart &first,
                                   int64_t start_b, int32_t start_w)
       : p(args), sh(share), part(first), b(start_b), w(share.w0) {
+    if (sh.descends) part.parts = -1;
     if (w >= sh.w1) return;
     int32_t from = start_w;  // first place of request b
     r = load_request(p, b);
@@ -215,7 +245,7 @@ struct Walk {
     }
   }
   // False past the last segment.
-  __device__ __forceinline__ bool next(Segment &sg) {
+  __host__ __device__ __forceinline__ bool next(Segment &sg) {
     while (w < sh.w1) {
       if (at >= n + unit_cost<ROWS>()) {  // a new unit
         if ((rt + 1) * ROWS < r.rows) {
@@ -250,7 +280,7 @@ struct Walk {
       if (sg.kind == kTail) {
         const int32_t last = unit0 + n - 1, big = sh.extra * (sh.share + 1);  // its last tile
         part.parts = (last < big ? last / (sh.share + 1) : sh.extra + (last - big) / sh.share) -
-                     static_cast<int32_t>(blockIdx.x) + 1;
+                     sh.cta + 1;
         part.tok0 = r.tok0;
         part.head = head;
         part.row0 = sg.row0;
@@ -271,8 +301,9 @@ __global__ void __launch_bounds__(256) tree_attn_join_parts_kernel(const TreePar
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int group = p.heads_per_kv;
   if (blockIdx.x == ctas) {
-    const int64_t c0 = min(max(static_cast<int64_t>(a.cu[0]), static_cast<int64_t>(0)), a.tokens);
-    const int64_t c1 = max(c0, min(static_cast<int64_t>(a.cu[a.requests]), a.tokens));
+    int64_t c0 = min(max(static_cast<int64_t>(a.cu[0]), static_cast<int64_t>(0)), a.tokens);
+    int64_t c1 = max(c0, min(static_cast<int64_t>(a.cu[a.requests]), a.tokens));
+    if (p.part[0].parts < 0) c0 = c1 = 0;  // no request has any
     const int64_t none = c0 + a.tokens - c1;  // tokens before the first and after the last request
     for (int64_t w = blockIdx.y * 8 + warp; w < none * a.heads; w += 8 * gridDim.y) {
       const int64_t at = w / a.heads, h = w - at * a.heads, t = at < c0 ? at : at - c0 + c1;
@@ -284,7 +315,7 @@ __global__ void __launch_bounds__(256) tree_attn_join_parts_kernel(const TreePar
     return;
   }
   const TreeAttnPart part = p.part[blockIdx.x];
-  if (part.parts == 0) return;
+  if (part.parts <= 0) return;
   const float2 *ml = reinterpret_cast<const float2 *>(p.partial +
                                                       static_cast<int64_t>(ctas) * 2 * ROWS * HD);
   // Part k: the tail slot of this CTA, then the head slots of the next ones.

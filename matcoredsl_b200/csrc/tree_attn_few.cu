@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(threads<kTma>())
   }
   grid_launch_dependents();
   const Share share = find_share<ROWS, threads<kTma>()>(
-      p, reinterpret_cast<int32_t *>(sm.p), true, &sm.start_b, &sm.start_w);
+      p, reinterpret_cast<uint32_t *>(sm.p), true, &sm.start_b, &sm.start_w);
 
   if (warp == WARPS) {
     // ---------------- tiles, queries and (TMA) keys and values ----------------

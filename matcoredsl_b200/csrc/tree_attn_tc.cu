@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
   constexpr int TILES = kPair ? 1 : 2;  // key tiles of a round
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem<HD, kPair> &sm = *reinterpret_cast<Smem<HD, kPair> *>(smem_raw);
-  int32_t *scan = reinterpret_cast<int32_t *>(sm.info);  // before the roles start
+  uint32_t *scan = &sm.info[0][0];  // before the roles start
   const TreeAttn &a = p.a;
   volatile int *abort_flag = &sm.abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -726,12 +726,13 @@ bool tree_attn_tc_ok(const TreeAttn &a, int dtype) {
   int64_t steps = a.q_s[0] | a.q_s[1] | a.o_s[0] | a.o_s[1];
   for (int i = 0; i < 3; ++i) steps |= a.k_s[i] | a.v_s[i];
   if (bases % 16 != 0 || steps % 8 != 0) return false;
-  // 32-bit numbers: rows, keys of a request, all key tiles, and the offsets of
-  // cache rows in 16 bytes (a cache of up to 64 GB).
+  // 32-bit numbers: rows, keys of a request, what all units cost (a tile begun and
+  // three more beside a unit's keys), and the offsets of cache rows in 16 bytes (a cache of
+  // up to 64 GB).
   const int64_t group = a.heads / a.kv_heads, rows = a.tokens * group;
   if (a.tokens * a.heads > 0x7fffffff || a.columns * a.block > 0x7fffff00) return false;
   const double tiles = (static_cast<double>(rows) / 16 + a.requests) * a.kv_heads *
-                       (static_cast<double>(a.columns) * a.block / BK + 1);
+                       (static_cast<double>(a.columns) * a.block / BK + 4);
   if (tiles > 0x7fffffff) return false;
   for (const int64_t *st : {a.k_s, a.v_s})
     if (st[0] / 8 > 0xffffffffLL || st[1] / 8 > 0xffffffffLL ||
