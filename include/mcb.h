@@ -689,7 +689,8 @@ MCB_API mcb_status mcb_rope_append_v1(const mcb_tensor *q_out, const mcb_tensor 
  * a token of no request) gives o = 0, lse = -inf; keys past the table's
  * columns and of table entries outside the cache are not seen. What is not
  * seen has no influence, NaN and infinities included. cu_new ascends; where it
- * descends anywhere, no token belongs to a request.
+ * descends anywhere, no token belongs to a request. Its entries may lie outside
+ * [0, T]: what is inside is computed as if the rest were there.
  * q, o and the caches share one type (bf16, f16, f32), dim <= 256. bf16 and
  * f16 with dim 64 or 128, 16-byte aligned bases and strides and a scale other
  * than 0 run on tensor cores (the weights rounded to the 16-bit type for the

@@ -79,20 +79,25 @@ __device__ __forceinline__ void cp_async_wait_all() {
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// One request's lengths, clipped to the tensors.
+// One request's lengths, clipped to the tensors. tok0 and rows are those of the tokens
+// inside [0, T). prefix is the position of the first new token (which the bits of a
+// mask count from) or, without a mask, of the first one inside: a row's own key
+// counts from there, and all rows see the keys before.
 struct Request {
-  int32_t tok0, rows, prefix, keys;  // rows: of the tokens inside [0, T)
+  int32_t tok0, rows, prefix, keys;
   bool descends;                     // cu_new does, at this request
 };
 __host__ __device__ __forceinline__ Request load_request(const TreeParams &p, int64_t b) {
   const TreeAttn &a = p.a;
   Request r;
   const int64_t c0 = a.cu[b], c1 = a.cu[b + 1], kv = max(0, a.kv_lens[b]);
-  const int64_t n = c0 >= 0 && c1 > c0 ? c1 - c0 : 0;
-  const int64_t in = max(static_cast<int64_t>(0), min(n, a.tokens - c0));
-  r.tok0 = static_cast<int32_t>(c0);
+  const int64_t first = max(c0, static_cast<int64_t>(0));
+  const int64_t in = max(static_cast<int64_t>(0), min(c1, a.tokens) - first);
+  r.tok0 = static_cast<int32_t>(first);
   r.rows = static_cast<int32_t>(in) * p.heads_per_kv;
-  r.prefix = static_cast<int32_t>(kv - n);
+  // (A mask has fewer than 2^31 bits a row: a token count past that is as good as that.)
+  r.prefix = static_cast<int32_t>(
+      kv - (a.mask ? min(c1 - c0, static_cast<int64_t>(0x7fffffff)) : c1 - first));
   r.keys = static_cast<int32_t>(min(kv, static_cast<int64_t>(p.most_keys)));
   r.descends = c1 < c0;
   return r;

@@ -2,7 +2,9 @@
 import numpy as np
 import pytest
 
+from tests import serving_ref as ref
 from tests.test_tree_attention_gpu import Case
+from tests.test_tree_attention_values_gpu import Coded
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +33,25 @@ def test_descending(mcb, dtype, heads, route, tree):
         out, lse = run(mcb, c, np.array(cu), route)
         assert (out == 0).all() and (lse == float("-inf")).all()
     c.check(mcb, route)
+
+
+@pytest.mark.parametrize("dtype,heads,route", ROUTES)
+@pytest.mark.parametrize("tree", [True, False])
+@pytest.mark.parametrize("cut", [(1, 0), (3, 2), (6, 0), (9, 7)])
+def test_requests_that_begin_before_the_first_token(mcb, dtype, heads, route, tree, cut):
+    """Entries below 0, and past the last token: what lies inside is computed as it would be with all
+    of them there."""
+    import torch
+    c = Coded([5] * 4, [300, 5, 140, 20], heads, 2, 128, 16, dtype, tree, seed=heads)
+    q, k, v, table, cu, kv, mask = c.args
+    here = slice(cut[0], 20 - cut[1])
+    out = torch.full_like(q[here], 7.0)
+    lse = torch.full(out.shape[:2], 7.0, device="cuda")
+    mcb.tree_attention(q[here], k, v, table, cu - cut[0], kv, None if mask is None else mask[here],
+                       scale=1.0, out=out, lse=lse)
+    if heads != 16 or cut != (9, 7):  # 8 heads a key head and one token a request are few rows
+        assert mcb.api.last_result.route == route
+    want, want_lse = c.want[here], c.want_lse[here]
+    tol = (ref.HALF_ULP[dtype] + 2.0 ** -22) * want.abs() + ref.TINY[dtype]
+    assert ((out.double() - want).abs() <= tol).all()
+    assert ((lse.double() - want_lse).abs() <= 2.0 ** -21 * want_lse.abs().clamp(min=1)).all()

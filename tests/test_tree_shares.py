@@ -102,6 +102,21 @@ def test_every_tile_is_taken_once(shares, rows, masked):
         check(shares, rows, 148, max(1, tokens - 5), 4, 2, 16, 250, masked, cu, kv - 50)
 
 
+@pytest.mark.parametrize("rows", [16, 128])
+@pytest.mark.parametrize("masked", [True, False])
+def test_requests_that_begin_before_the_first_token(shares, rows, masked):
+    """Their tokens from the first one on are shared out like all others."""
+    rng = np.random.default_rng(rows)
+    for cut in (1, 3, 17, 70):
+        new = rng.integers(0, 40, 7)
+        kv = new + rng.integers(0, 3000, 7)
+        cu = np.concatenate([[0], np.cumsum(new)])
+        check(shares, rows, 148, int(cu[-1]) - cut, 4, 2, 16, 100, masked, cu - cut, kv)
+    far = np.array([-2 ** 31, 5, 2 ** 31 - 1])
+    for tokens in (3, 9):
+        check(shares, rows, 148, tokens, 4, 2, 16, 100, masked, far, np.array([300, 1000]))
+
+
 @pytest.mark.parametrize("rows", [16, 32, 128, 256])
 @pytest.mark.parametrize("masked", [True, False])
 def test_where_cu_new_descends_nothing_is_shared_out(shares, rows, masked):
