@@ -11,6 +11,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <string.h>
 
 namespace mcb {
 
@@ -444,10 +445,37 @@ __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-__device__ __forceinline__ float fmax3(float a, float b, float c) {
+__host__ __device__ __forceinline__ float fmax3(float a, float b, float c) {
+#if defined(__CUDA_ARCH__)
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
+#else
+  return fmaxf(a, fmaxf(b, c));
+#endif
+}
+// The largest of N f32 values (their bits): four chains of three-input maxima, two
+// values a step.
+template <int N>
+__host__ __device__ __forceinline__ float max_of(const uint32_t (&s)[N]) {
+  static_assert(N >= 8 && N % 8 == 0, "eight values begin the chains, eight a step");
+  auto at = [&](int i) -> float {
+#if defined(__CUDA_ARCH__)
+    return __uint_as_float(s[i]);
+#else
+    float f;
+    memcpy(&f, &s[i], sizeof(f));
+    return f;
+#endif
+  };
+  float m4[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) m4[j] = fmaxf(at(2 * j), at(2 * j + 1));
+#pragma unroll
+  for (int i = 8; i < N; i += 8)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m4[j] = fmax3(m4[j], at(i + 2 * j), at(i + 2 * j + 1));
+  return fmax3(m4[0], m4[1], fmaxf(m4[2], m4[3]));
 }
 
 __device__ __forceinline__ float tanh_fast(float x) {

@@ -698,16 +698,7 @@ __global__ void __launch_bounds__(THREADS2, 1)
         tc_fence_before();
         mbar_arrive(&sm.s_free[g]);
         ++s_cnt;
-        // Row max: four chains of three-input max, two scores per step.
-        float m4[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) m4[i] = __uint_as_float(s[i]);
-#pragma unroll
-        for (int i = 4; i < 128; i += 8)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            m4[j] = fmax3(m4[j], __uint_as_float(s[i + 2 * j]), __uint_as_float(s[i + 2 * j + 1]));
-        const float mx = fmax3(m4[0], m4[1], fmaxf(m4[2], m4[3]));
+        const float mx = max_of(s);
         bool need = false;
         if (t == 0) {
           m_ref = mx;

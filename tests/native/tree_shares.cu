@@ -4,29 +4,13 @@
 //   cu_new[requests + 1]  kv_lens[requests]
 // and prints a line for each segment: cta kind b head row0 nrows tok0 prefix keys tile0 ntiles,
 // then for each CTA: part cta parts tok0 head row0 nrows.
-#include <sys/mman.h>
-#include <unistd.h>
-
 #include <cstdio>
-#include <cstring>
-#include <vector>
 
+#include "fence.h"
 #include "tree_attn.cuh"
 
 using namespace mcb;
 using namespace mcb::tree;
-
-// A copy of x whose end is the end of a page, with nothing behind it.
-static int32_t *fenced(const std::vector<int32_t> &x) {
-  const size_t page = static_cast<size_t>(sysconf(_SC_PAGESIZE)), bytes = x.size() * sizeof(int32_t);
-  const size_t room = (bytes + page - 1) / page * page;
-  char *base = static_cast<char *>(
-      mmap(nullptr, room + page, PROT_READ | PROT_WRITE, MAP_PRIVATE | MAP_ANONYMOUS, -1, 0));
-  if (base == MAP_FAILED || mprotect(base + room, page, PROT_NONE) != 0) return nullptr;
-  char *at = base + room - bytes;
-  std::memcpy(at, x.data(), bytes);
-  return reinterpret_cast<int32_t *>(at);
-}
 
 template <int ROWS>
 static void run(const TreeParams &p, int threads, int grid) {

@@ -1,28 +1,19 @@
 """CPU: the attention over a paged cache shares every unit's key tiles out once, whatever the lengths
 say, and reads no length that is not there. The functions that the kernels run on the device are
 compiled for the host (tests/native/tree_shares.cu)."""
-import os
 import subprocess
 
 import numpy as np
 import pytest
 
-ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-NVCC = os.environ.get("MCB_NVCC", "/usr/local/cuda/bin/nvcc")
+from tests.native_util import compile_native
+
 COST = {16: 1, 32: 1, 128: 3, 256: 3}
 
 
 @pytest.fixture(scope="module")
 def shares(tmp_path_factory):
-    if not os.path.exists(NVCC):
-        pytest.skip("no nvcc")
-    out = str(tmp_path_factory.mktemp("native") / "tree_shares")
-    subprocess.run(
-        [NVCC, "-gencode", "arch=compute_100a,code=sm_100a", "-O1", "-std=c++17",
-         "--expt-relaxed-constexpr", "-ccbin", "/usr/bin/g++", "-I", os.path.join(ROOT, "include"),
-         "-I", os.path.join(ROOT, "matcoredsl_b200", "csrc"),
-         os.path.join(ROOT, "tests", "native", "tree_shares.cu"), "-o", out],
-        check=True, capture_output=True, text=True)
+    out = compile_native("tree_shares", tmp_path_factory.mktemp("native"))
 
     def run(rows, threads, grid, tokens, group, kv_heads, block, columns, masked, cu, kv):
         numbers = [rows, threads, grid, tokens, group, kv_heads, block, columns, int(masked), len(kv),
