@@ -2270,7 +2270,10 @@ mcb_status tree_attention_impl(const mcb_tensor *o, const mcb_tensor *lse, const
   p.table = i32(table);
   p.cu = i32(cu);
   p.kv_lens = i32(kv_lens);
-  p.mask = mask ? static_cast<const uint32_t *>(mask->data) : nullptr;
+  // (A mask of no words may have no address. It is a mask all the same, and none of it is read.)
+  p.mask = !mask                ? nullptr
+           : mask->dims[1] == 0 ? static_cast<const uint32_t *>(cu->data)
+                                : static_cast<const uint32_t *>(mask->data);
   p.tokens = T;
   p.requests = B;
   p.heads = static_cast<int32_t>(H);

@@ -1,4 +1,5 @@
-"""Attention of drafted tokens over a paged cache: what cu_new may hold, the same on all three routes."""
+"""Attention of drafted tokens over a paged cache: what cu_new and the mask may hold, the same on all
+three routes."""
 import numpy as np
 import pytest
 
@@ -55,3 +56,17 @@ def test_requests_that_begin_before_the_first_token(mcb, dtype, heads, route, tr
     tol = (ref.HALF_ULP[dtype] + 2.0 ** -22) * want.abs() + ref.TINY[dtype]
     assert ((out.double() - want).abs() <= tol).all()
     assert ((lse.double() - want_lse).abs() <= 2.0 ** -21 * want_lse.abs().clamp(min=1)).all()
+
+
+@pytest.mark.parametrize("dtype,heads,route", ROUTES)
+def test_a_mask_of_no_words(mcb, dtype, heads, route):
+    """It has no bit set: no token sees a new one, its own included."""
+    import torch
+    c = Case([5] * 4, [300, 5, 140, 20], heads, 2, 128, 16, dtype)
+    c.mask = np.zeros((20, 1), np.int64)
+    want, want_lse = run(mcb, c, c.cu, route)
+    c.mask = np.zeros((20, 0), np.int64)
+    out, lse = run(mcb, c, c.cu, route)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    assert (out[5:10] == 0).all() and (lse[5:10] == float("-inf")).all()  # no prefix either
+    assert (lse[:5] > 0).all()
