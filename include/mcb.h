@@ -669,7 +669,8 @@ MCB_API mcb_status mcb_rope_v1(const mcb_tensor *q_out, const mcb_tensor *k_out,
 /* The same with the turned k and v [T, kv_heads, dim] written to row slots[t]
  * of the caches [blocks, block, kv_heads, dim] of the same type (any strides
  * with unit innermost; blocks * block < 2^31). A slot outside the cache (-1 by
- * convention) writes nothing; two tokens with one slot leave either. */
+ * convention) writes nothing; two tokens with one slot leave either. The caches
+ * may be views of one tensor that share no element. */
 MCB_API mcb_status mcb_rope_append_v1(const mcb_tensor *q_out, const mcb_tensor *k_cache,
                                       const mcb_tensor *v_cache, const mcb_tensor *q,
                                       const mcb_tensor *k, const mcb_tensor *v,

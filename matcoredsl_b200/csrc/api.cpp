@@ -1987,20 +1987,43 @@ bool same_place(const mcb_tensor *a, const mcb_tensor *b) {
       return false;
   return true;
 }
-// Whether two [T, heads, dim] views share an element, for views whose rows
-// interleave too (q, k and v of one packed projection): with equal row strides
-// they are apart when each row's spans are, modulo the stride.
+// Whether two views whose spans overlap share an element: exact for views of one type and rank
+// with equal strides (q, k and v of one packed projection, K and V caches of one tensor),
+// else yes.
+struct SharedDim {
+  int64_t stride, a, b;  // extents in either view
+};
+// Whether sum stride * (i_a - i_b) over the dims from `d` on takes the value `off` (elements).
+bool reaches(const SharedDim *d, int n, int64_t off) {
+  if (n == 0) return off == 0;
+  // What the smaller strides add: from -low_b to low_a.
+  int64_t low_a = 0, low_b = 0;
+  for (int i = 1; i < n; ++i) {
+    low_a += (d[i].a - 1) * d[i].stride;
+    low_b += (d[i].b - 1) * d[i].stride;
+  }
+  auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
+  const int64_t first = std::max(floor_div(off - low_a + d->stride - 1, d->stride), 1 - d->b);
+  const int64_t last = std::min(floor_div(off + low_b, d->stride), d->a - 1);
+  if (last - first > 4) return true;  // strides that do not nest: not looked at further
+  for (int64_t k = first; k <= last; ++k)
+    if (reaches(d + 1, n - 1, off - k * d->stride)) return true;
+  return false;
+}
 bool views_overlap(const mcb_tensor *a, const mcb_tensor *b) {
   if (!overlaps(a, b)) return false;
-  if (a->rank != 3 || b->rank != 3 || a->dtype != b->dtype || a->strides[0] != b->strides[0])
-    return true;
-  const int64_t es = static_cast<int64_t>(dtype_size(a->dtype)), row = a->strides[0];
-  auto width = [](const mcb_tensor *t) { return (t->dims[1] - 1) * t->strides[1] + t->dims[2]; };
-  if (width(a) > row || width(b) > row) return true;
+  if (a->rank != b->rank || a->dtype != b->dtype) return true;
+  SharedDim d[MCB_MAX_RANK];
+  int n = 0;
+  for (uint32_t i = 0; i < a->rank; ++i) {
+    if (a->dims[i] == 1 && b->dims[i] == 1) continue;
+    if (a->dims[i] > 1 && b->dims[i] > 1 && a->strides[i] != b->strides[i]) return true;
+    d[n++] = {a->dims[i] > 1 ? a->strides[i] : b->strides[i], a->dims[i], b->dims[i]};
+  }
+  std::sort(d, d + n, [](const SharedDim &x, const SharedDim &y) { return x.stride > y.stride; });
+  const int64_t es = static_cast<int64_t>(dtype_size(a->dtype));
   const int64_t apart = static_cast<const char *>(b->data) - static_cast<const char *>(a->data);
-  if (apart % es != 0) return true;
-  const int64_t off = ((apart / es) % row + row) % row;
-  return !(off >= width(a) && off + width(b) <= row);
+  return apart % es != 0 || reaches(d, n, apart / es);
 }
 const int32_t *i32(const mcb_tensor *t) { return t ? static_cast<const int32_t *>(t->data) : nullptr; }
 int32_t *i32_out(const mcb_tensor *t) { return static_cast<int32_t *>(t->data); }
@@ -2174,7 +2197,7 @@ mcb_status rope_impl(const mcb_tensor *q_out, const mcb_tensor *k_out, const mcb
     }
   }
   if (views_overlap(q_out, k_out) || (append && (views_overlap(q_out, v_cache) ||
-                                                 overlaps(k_out, v_cache))))
+                                                 views_overlap(k_out, v_cache))))
     return MCB_STATUS_ALIAS_VIOLATION;
   Call call(exec);
   if ((s = call.begin(false))) return s;
