@@ -135,3 +135,26 @@ def test_short_units_follow_each_other(mcb, tree, rows):
     for _ in range(100):
         mcb.tree_attention(*c.args, scale=1.0, out=again, lse=again_lse)
         assert torch.equal(again, got) and torch.equal(again_lse, lse)
+
+
+@pytest.mark.parametrize("dim,new,block", [(128, 1, 256), (128, 4, 16), (64, 1, 128)])
+def test_few_rows_call_after_call(mcb, dim, new, block):
+    """Keys and values from L2 come so fast that a stage is written again as soon as it is given back:
+    whoever still reads it then gets rows of the next keys. One call in some thousands did."""
+    import torch
+    g = torch.Generator(device="cuda")
+    g.manual_seed(dim + new)
+    n, pool = 300, 640 // (block // 16 if block > 16 else 1)
+    kv = (new + torch.rand(n, generator=g, device="cuda") * 4000).int()
+    table = torch.randint(0, pool, (n, 4096 // block + 1), generator=g, device="cuda").int()
+    rand = lambda *s: torch.randn(*s, generator=g, device="cuda").to(torch.float16)  # noqa: E731
+    k, v = (rand(pool, block, 8, dim) for _ in range(2))
+    args = (rand(n * new, 8 * (8 if new == 1 else 2), dim), k, v, table,
+            torch.arange(0, n * new + 1, new, dtype=torch.int32, device="cuda"), kv)
+    want = mcb.tree_attention(*args)
+    assert mcb.api.last_result.route == FEW
+    out, wrong = torch.empty_like(want), torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(6000):
+        mcb.tree_attention(*args, out=out)
+        wrong += (out != want).any()
+    assert int(wrong) == 0
