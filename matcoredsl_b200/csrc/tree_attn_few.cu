@@ -24,8 +24,8 @@
 // each key of a tile lies and copies the queries and, where a cache block is a
 // whole box of a tensor map (8 rows or more, and a divisor or multiple of 128),
 // keys and values by TMA. Blocks of other sizes are copied row by row with
-// cp.async by eight more warps: 64 requests of up to 8192 keys take 211 us with blocks of
-// 24, 174 with blocks of 16 (1.09 GB at 6.3 TB/s). (The compute warps issuing those copies themselves,
+// cp.async by eight more warps: 64 requests of up to 8192 keys take 205 us with blocks of
+// 24, 177 with blocks of 16 (1.09 GB at 6.2 TB/s). (The compute warps issuing those copies themselves,
 // between their products, took 2.4 us a tile: 1.6 thousand cycles of the copies'
 // own.)
 #include "tree_attn.cuh"
@@ -36,7 +36,7 @@ using namespace tree;
 
 constexpr int WARPS = 8;
 constexpr int COMPUTE = WARPS * 32;
-constexpr int COPIERS = 256;  // threads of the row-by-row copies (128: 270 us where these take 211)
+constexpr int COPIERS = 256;  // threads of the row-by-row copies (128: 270 us where these took 211)
 template <bool kTma>
 constexpr int threads() {
   return COMPUTE + 32 + (kTma ? 0 : COPIERS);
@@ -327,8 +327,8 @@ __global__ void __launch_bounds__(threads<kTma>())
   // This thread is done with a half tile. TMA will write its place through the async
   // proxy, which only a proxy fence orders behind this thread's reads (and writes) of it:
   // without it, one call in 4000 (of 300 requests whose keys and values lie in L2) had
-  // rows of later keys among the values. (Decoding of 64 requests: 174 us with it, 180
-  // without.)
+  // rows of later keys among the values. (Decoding of 64 requests with two CTAs an SM:
+  // 177 us with it, 180 without; with one CTA 198 and 187.)
   auto release = [&](uint64_t *bar) {
     if (kTma) fence_async_smem();
     mbar_arrive(bar);
@@ -634,12 +634,12 @@ __global__ void __launch_bounds__(threads<kTma>())
 // Row tiles of 16 that a CTA takes, 0 where tcgen05 is the faster. By the rows that a
 // request has on average; of drafted tokens some requests have more than that, and
 // one whose rows do not fit reads its context twice, so a tile counts as 12 rows then.
-//   one tile: 64 requests of 4 rows, up to 8192 keys 189 us (304 on tcgen05, 230 with two
-//     tiles); 32 of 16 rows 102 (112); of 9 to 20 rows 243 (221), hence 12.
-//   two tiles: 256 requests of 16 to 32 rows, up to 1000 keys 183 us (225 on tcgen05, whose
-//     units cost three tiles more than their keys), 2000 keys 288 (317), 4000 keys 487
-//     (461); 64 requests with 4000 keys 142 (125), 8192 keys 245 (228); of 20 to 40 rows
-//     with 1000 keys 74 (68). So they are taken where no context can pass 2048 keys.
+//   one tile: 64 requests of 4 rows, up to 8192 keys 177 us (216 on tcgen05, 247 with two
+//     tiles); 32 of 16 rows 99 (107); of 12 to 20 rows 217 (215), hence 12.
+//   two tiles: 256 requests of 16 to 32 rows, up to 1000 keys 189 us (226 on tcgen05, whose
+//     units cost three tiles more than their keys), 2000 keys 301 (322), 4000 keys 514
+//     (482); 64 requests with 4000 keys 150 (132), 8192 keys 259 (225); of 20 to 40 rows
+//     with 1000 keys 72 (70). So they are taken where no context can pass 2048 keys.
 int row_tiles(const TreeAttn &a) {
   const int64_t rows = a.tokens * (a.heads / a.kv_heads);
   const int64_t tile = a.tokens == a.requests ? 16 : 12;
@@ -648,13 +648,15 @@ int row_tiles(const TreeAttn &a) {
 }
 // CTAs per SM: two where they fit (228 KB of shared memory, 1 KB kept per CTA) and there
 // are enough units, else contexts are cut into more parts than the second CTA is worth.
-// Head size 128, 8 key heads, up to 8192 keys: 1 request 26.6 us with one, 35.4 with two;
-// 32 requests 99.4 both; 64 requests 187 and 181, up to 1000 keys 43 and 37. Head size
-// 64: 1 request 24.6 and 32.3, 4 requests 25.1 and 27.0, 8 requests 32.7 and 29.0.
+// Head size 128, 8 key heads, up to 8192 keys: 1 request 24.6 us with one, 33 with two; 8
+// requests 41 both; 20 requests 73.7 and 68.5, 32 requests 107 and 99, 64 requests 198
+// and 177; up to 1000 keys 16 requests 21.5 both, 24 requests 24.6 and 22.6, 64
+// requests 45 and 37. Head size 64: 1 request 28.6 and 35, 4 requests 26.6 both, 8
+// requests 32.8 and 30.4.
 template <int HD, int MT, bool kTma>
 int per_sm(const TreeAttn &a, int sms) {
   if (2 * (sizeof(Smem<HD, MT, kTma>) + 1024) > 233472) return 1;
-  return a.requests * a.kv_heads >= (HD == 128 ? 2 * sms : sms / 4) ? 2 : 1;
+  return a.requests * a.kv_heads >= (HD == 128 ? sms : sms / 4) ? 2 : 1;
 }
 
 // Rows of a TMA box, 0 where blocks are no whole boxes.

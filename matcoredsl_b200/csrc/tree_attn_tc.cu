@@ -3,7 +3,7 @@
 // (The mathematics and the masks: tree_attn.cu.)
 //
 // Bound: HBM up to about 255 rows a key head, the tensor cores above. Two contexts of
-// 131072 and 0 keys, 56 rows by 8 key heads, f16: 113 us, 537 MB at 4.8 TB/s. 24 trees of
+// 131072 and 0 keys, 56 rows by 8 key heads, f16: 104 us, 537 MB at 5.2 TB/s. 24 trees of
 // 32 to 64 tokens by 8 heads over up to 6000 keys: 107 us, 61 GFLOP at 570 TFLOP/s, the
 // softmax (about 1850 cycles per 64 keys) behind it.
 //
