@@ -689,7 +689,8 @@ MCB_API mcb_status mcb_rope_append_v1(const mcb_tensor *q_out, const mcb_tensor 
  * plain decoding. heads is a multiple of kv_heads. A row that sees no key (and
  * a token of no request) gives o = 0, lse = -inf; keys past the table's
  * columns and of table entries outside the cache are not seen. What is not
- * seen has no influence, NaN and infinities included. cu_new ascends; where it
+ * seen has no influence, NaN and infinities included (an infinite value that is
+ * seen with a weight too small for f32 gives infinity or NaN). cu_new ascends; where it
  * descends anywhere, no token belongs to a request. Its entries may lie outside
  * [0, T]: what is inside is computed as if the rest were there.
  * q, o and the caches share one type (bf16, f16, f32), dim <= 256. bf16 and
@@ -723,7 +724,9 @@ MCB_API mcb_status mcb_tree_attention_v1(const mcb_tensor *o, const mcb_tensor *
  *                       x = x + its bias_values entry (its last, if several)
  *   bit v of row r of allowed [R, ceil(V/32)] (i32) clear: x = -inf
  * Any of repetition, presence, frequency [R] f32, the three bias tensors
- * (together) and allowed may be NULL. Ids outside [0, V) are ignored. */
+ * (together) and allowed may be NULL. Ids outside [0, V) are ignored; a history or
+ * list is cut to the entries that there are, and the prompt counts from the first
+ * of them. */
 MCB_API mcb_status mcb_adjust_logits_v1(const mcb_tensor *out, const mcb_tensor *logits,
                                         const mcb_tensor *token_ids, const mcb_tensor *cu_tokens,
                                         const mcb_tensor *prompt_lens,

@@ -84,7 +84,7 @@ bool encode_tmap_5d(CUtensorMap *map, CUtensorMapDataType dtype, const void *bas
     if (i > 0) st[i - 1] = dims[i] > 1 ? strides[i - 1] : 16;
   }
   // No promotion past 128 bytes: where a head's row has no more, the next head's would
-  // be read with it (64 requests of head size 64: 23% more bytes, 132 us instead of 103).
+  // be read with it (64 requests of head size 64: 330 MB instead of 268, a quarter more time).
   return fn(map, dtype, 5, const_cast<void *>(base), d, st, b, estr,
             CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;

@@ -4,7 +4,7 @@
 //
 // Bound: HBM up to about 255 rows a key head, the tensor cores above. Two contexts of
 // 131072 and 0 keys, 56 rows by 8 key heads, f16: 104 us, 537 MB at 5.2 TB/s. 24 trees of
-// 32 to 64 tokens by 8 heads over up to 6000 keys: 107 us, 61 GFLOP at 570 TFLOP/s, the
+// 32 to 64 tokens by 8 heads over up to 6000 keys: 109 us, 61 GFLOP at 560 TFLOP/s, the
 // softmax (about 1850 cycles per 64 keys) behind it.
 //
 // A unit is one request, one key head and up to ROWS of the request's rows
@@ -697,7 +697,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const Params p
 
 bool pair_of(const TreeAttn &a) {
   // Two row halves per CTA when a request has more than 128 rows on average: 24 trees of
-  // 32 to 64 tokens by 8 heads 107 us, 147 us with 128 rows a CTA, which read each
+  // 32 to 64 tokens by 8 heads 109 us, 147 us with 128 rows a CTA, which read each
   // context twice; below that the second half would be empty.
   return a.tokens * (a.heads / a.kv_heads) > 128 * a.requests;
 }

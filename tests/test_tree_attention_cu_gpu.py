@@ -70,3 +70,21 @@ def test_a_mask_of_no_words(mcb, dtype, heads, route):
     assert torch.equal(out, want) and torch.equal(lse, want_lse)
     assert (out[5:10] == 0).all() and (lse[5:10] == float("-inf")).all()  # no prefix either
     assert (lse[:5] > 0).all()
+
+
+@pytest.mark.parametrize("dtype,heads,route", ROUTES)
+@pytest.mark.parametrize("new", [True, False])
+def test_an_infinite_value_whose_weight_is_too_small(mcb, dtype, heads, route, new):
+    """Seen all the same: infinity or not a number in its place, nothing elsewhere. Among the new
+    tokens' values and among those before them."""
+    import torch
+    c = Case([5] * 4, [300, 5, 140, 20], heads, 2, 128, 16, dtype, tree=False)
+    c.q[:] = 1.0
+    pos = 295 if new else 200
+    blk = int(c.table[0, pos // 16])
+    c.k[blk, pos % 16] = -64.0  # a score 700 below the others'
+    c.v[blk, pos % 16, :, ::3] = float("inf")
+    out, lse = run(mcb, c, c.cu, route)
+    assert not torch.isfinite(out[:5, :, ::3]).any()
+    out[:5, :, ::3] = 0.0
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
